@@ -668,8 +668,6 @@ int gpx_init(int device, gpx_ctx** out) {
     return -3;
   }
   {
-    int lo = 0, hi = 0; // numerically lower = higher priority
-    GPX_HIP(ctx, hipDeviceGetStreamPriorityRange(&lo, &hi));
     // The library's switches (12 in all, this list + GPX_ROCTX, GPX_SWEEP_BATCH, GPX_NODE_TRANSPORT, GPX_RANK_FILE_TIMEOUT):
     // each selects the ONE alternate of a kernel / schedule that the bit-identity tests compare the default against.
     // Everything else rounds 1 - 3 measured and rejected (CU reservations, early diagonal, split U1 / far updates,
@@ -688,9 +686,11 @@ int gpx_init(int device, gpx_ctx** out) {
       }
     }
     if (const char* e = getenv("GPX_TAIL_TILES")) ctx->tail_tiles = atoi(e);
-    GPX_HIP(ctx, hipStreamCreateWithPriority(&ctx->stream, hipStreamNonBlocking, lo));
-    GPX_HIP(ctx, hipStreamCreateWithPriority(&ctx->pstream, hipStreamNonBlocking, hi));
-    GPX_HIP(ctx, hipStreamCreateWithPriority(&ctx->xstream, hipStreamNonBlocking, lo));
+    // all of the default priority: a chain kernel is placed early because it FITS beside the trailing update
+    // (potf2_slim.h), which a stream's priority does not change, and work on streams of unequal priority has hung
+    GPX_HIP(ctx, hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking));
+    GPX_HIP(ctx, hipStreamCreateWithFlags(&ctx->pstream, hipStreamNonBlocking));
+    GPX_HIP(ctx, hipStreamCreateWithFlags(&ctx->xstream, hipStreamNonBlocking));
     GPX_HIP(ctx, hipEventCreateWithFlags(&ctx->evD, hipEventDisableTiming));
     if (const char* e = getenv("GPX_POTF2")) {
       if (gpx_debug_set_potf2(ctx, e) != 0) return -1;

@@ -170,8 +170,8 @@ struct ProfAcc {
 struct gpx_ctx {
   int device = -1;
   hipStream_t stream = nullptr;  // main stream (API copies, trailing updates)
-  hipStream_t pstream = nullptr; // high-priority panel stream (lookahead)
-  hipStream_t xstream = nullptr; // side stream, lowest priority: work with time to spare beside a chain (the L^-T trees of
+  hipStream_t pstream = nullptr; // panel stream (lookahead)
+  hipStream_t xstream = nullptr; // side stream: work with time to spare beside a chain (the L^-T trees of
                                  // the sparse path while the next factorisation's chain or the tall solve runs; sparse.hip)
   hipStream_t s = nullptr;       // stream the launch helpers currently target
   // diagonal-block kernel (potf2.hip): GPX_POTF2 = slim (default: placed at once beside two resident trailing-update
