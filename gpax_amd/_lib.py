@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import threading
 from typing import Optional, Tuple
 
 import numpy as np
@@ -33,6 +34,14 @@ class GpxError(RuntimeError):
     pass
 
 
+class PoolScores(C.Structure):
+    """gpx_scores (include/gpx.h)."""
+    _fields_ = [("d_scores", C.c_void_p), ("pools", C.c_int64), ("rows", C.c_int64), ("candidates", C.c_int64),
+                ("scores_stride", C.c_int64 * 3), ("d_mask", C.c_void_p), ("mask_stride", C.c_int64 * 3),
+                ("d_lengths", C.c_void_p), ("lengths_stride", C.c_int64 * 2), ("d_temperatures", C.c_void_p),
+                ("temperatures_stride", C.c_int64 * 2), ("temperature", C.c_double), ("dtype", C.c_int), ("lengths_64", C.c_int)]
+
+
 def lib_path() -> str:
     return _LIB_PATH
 
@@ -48,7 +57,7 @@ def load_library() -> C.CDLL:
             "(or `make -C gpax_amd/csrc`). gpax_amd has no CPU fallback."
         )
     lib = C.CDLL(_LIB_PATH)
-    vp = C.c_void_p
+    vp, i64, scp = C.c_void_p, C.c_int64, C.POINTER(PoolScores)
     sig = {
         "gpx_init": (C.c_int, [C.c_int, C.POINTER(vp)]),
         "gpx_device_count": (C.c_int, []),
@@ -119,6 +128,17 @@ def load_library() -> C.CDLL:
                                              _dp, C.c_int, C.c_int, C.c_double, _dp, C.c_int, _dp, _dp, _ip, _dp,
                                              C.c_int, C.c_int]),
         "gpx_shard_range": (C.c_int, [C.c_int, C.c_int, C.c_int, _ip, _ip]),
+        "gpx_choice_workspace": (i64, [i64, i64, i64, C.c_int, C.c_int]),
+        "gpx_choice_logprobs": (C.c_int, [vp, scp, vp, i64, C.c_int, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
+        "gpx_choice_logprobs_grad": (C.c_int, [vp, scp, vp, i64, vp, vp, C.c_int, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "gpx_pool_weights_workspace": (i64, [i64, i64, i64, C.c_int]),
+        "gpx_pool_weights": (C.c_int, [vp, scp, vp, vp, C.c_double, vp, vp, i64, vp]),
+        "gpx_pool_evict": (C.c_int, [vp, C.c_int, i64, i64, vp, vp, C.c_int, i64, i64, i64, i64, vp, vp, vp, C.c_int,
+                                     C.POINTER(vp), C.POINTER(vp), C.POINTER(i64), vp]),
+        "gpx_scratch": (C.c_int, [vp, i64, C.POINTER(vp)]),
+        "gpx_upload": (C.c_int, [vp, vp, vp, i64]),
+        "gpx_download": (C.c_int, [vp, vp, vp, i64]),
+        "gpx_stream": (vp, [vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)  # AttributeError here = header/library mismatch: fail loudly
@@ -135,7 +155,9 @@ EXPORTED_SYMBOLS = (
     "gpx_profile_reset gpx_profile_read gpx_profile_read_bytes gpx_debug_set_potf2 gpx_debug_set_lat_gemm gpx_nuts_transition gpx_nuts_potential gpx_debug_pcg64_doubles gpx_debug_set_serialise_trailing gpx_debug_gemm_time gpx_debug_tile_list gpx_time_stage gpx_sweep_resident gpx_sweep_stats gpx_mfma_f64_peak gpx_gemm_nt "
     "gpx_potrf gpx_node_init gpx_node_destroy gpx_node_last_error gpx_node_info gpx_node_last_shares gpx_predict_sweep_multi "
     "gpx_rank_unique_id gpx_rank_init gpx_rank_destroy gpx_rank_last_error gpx_rank_info gpx_rank_device_pci gpx_rank_collective_calls gpx_rank_barrier gpx_rank_calibrate gpx_shard_ranges_weighted "
-    "gpx_rank_allreduce_max gpx_rank_bcast gpx_rank_predict_sweep gpx_shard_range"
+    "gpx_rank_allreduce_max gpx_rank_bcast gpx_rank_predict_sweep gpx_shard_range "
+    "gpx_choice_workspace gpx_choice_logprobs gpx_choice_logprobs_grad gpx_pool_weights_workspace gpx_pool_weights gpx_pool_evict "
+    "gpx_scratch gpx_upload gpx_download gpx_stream"
 ).split()
 
 
@@ -209,6 +231,7 @@ class Engine:
         self._diag_key = None
         self._train_owner = None
         self._train_version = None
+        self._pool_lock = threading.Lock()  # calls on one context are one at a time (the pool operators take it)
 
     # -- plumbing -----------------------------------------------------------------------------
     def _check(self, rc: int, what: str):
@@ -466,6 +489,50 @@ class Engine:
                                                 _ptr(Xu), Xu.shape[0], _ptr(yres), _ptr(Xnew), Ms, float(noise_p),
                                                 _ptr(mean), _ptr(cov), _ptr(var), C.byref(info)), "gpx_sgp_posterior")
         return mean, cov, var, info.value
+
+    # -- operators over a pool of candidates (gpax_amd/acquisition/pool.py prepares their arguments) ----------------
+    # Addresses are device addresses (ints, 0 = none) on this engine's GPU; `stream` is a stream of it.  Nothing waits.
+    def choice_logprobs(self, scores: PoolScores, choices: int, nchoices: int, top: int, logprobs: int, entropy: int,
+                        logsumexp: int, stats: int, top_indices: int, top_logprobs: int, workspace: int,
+                        workspace_bytes: int, stream: int) -> None:
+        self._check(self._lib.gpx_choice_logprobs(self._ctx, C.byref(scores), choices, nchoices, top, logprobs, entropy,
+                                                  logsumexp, stats, top_indices, top_logprobs, workspace, workspace_bytes,
+                                                  stream), "gpx_choice_logprobs")
+
+    def choice_logprobs_grad(self, scores: PoolScores, choices: int, nchoices: int, logprobs: int, grad_logprobs: int,
+                             top: int, top_indices: int, grad_top: int, entropy: int, stats: int, grad_entropy: int,
+                             grad_logsumexp: int, grad_scores: int, stream: int) -> None:
+        self._check(self._lib.gpx_choice_logprobs_grad(self._ctx, C.byref(scores), choices, nchoices, logprobs, grad_logprobs,
+                                                       top, top_indices, grad_top, entropy, stats, grad_entropy,
+                                                       grad_logsumexp, grad_scores, stream), "gpx_choice_logprobs_grad")
+
+    def pool_weights(self, scores: PoolScores, row_weights: int, weights: int, decay: float, out: int, workspace: int,
+                     workspace_bytes: int, stream: int) -> None:
+        self._check(self._lib.gpx_pool_weights(self._ctx, C.byref(scores), row_weights, weights, decay, out, workspace,
+                                               workspace_bytes, stream), "gpx_pool_weights")
+
+    def pool_evict(self, dtype: int, pools: int, candidates: int, weights: int, lengths: int, lengths_64: bool,
+                   lengths_stride: int, budget: int, first: int, recent: int, indices: int, new_lengths: int,
+                   weights_out: int, payload: list, payload_out: list, row_bytes: list, stream: int) -> None:
+        n = len(payload)
+        self._check(self._lib.gpx_pool_evict(self._ctx, dtype, pools, candidates, weights, lengths, int(lengths_64),
+                                             lengths_stride, budget, first, recent, indices, new_lengths, weights_out, n,
+                                             (C.c_void_p * n)(*payload), (C.c_void_p * n)(*payload_out),
+                                             (C.c_int64 * n)(*row_bytes), stream), "gpx_pool_evict")
+
+    def scratch(self, nbytes: int) -> int:
+        out = C.c_void_p()
+        self._check(self._lib.gpx_scratch(self._ctx, nbytes, C.byref(out)), "gpx_scratch")
+        return out.value
+
+    def upload(self, address: int, a: np.ndarray) -> None:
+        self._check(self._lib.gpx_upload(self._ctx, address, a.ctypes.data, a.nbytes), "gpx_upload")
+
+    def download(self, a: np.ndarray, address: int) -> None:
+        self._check(self._lib.gpx_download(self._ctx, a.ctypes.data, address, a.nbytes), "gpx_download")
+
+    def stream(self) -> int:
+        return self._lib.gpx_stream(self._ctx) or 0
 
     # -- measurement ----------------------------------------------------------------------------
     def profile_enable(self, on: bool):
@@ -861,6 +928,23 @@ def set_engine(engine) -> None:
     global _default_engine, _sweep_pool
     _default_engine = engine
     _sweep_pool = []
+
+
+_device_engines: dict = {}
+_device_engines_lock = threading.Lock()
+
+
+def get_device_engine(device: int) -> Engine:
+    """An engine on GPU `device` for operators on arrays that live there.  The default engine where it is that GPU's, else
+    one kept beside it: the models' engine stays the default whatever device such a call is for."""
+    e = _default_engine
+    if isinstance(e, Engine) and e.device == device:
+        return e
+    with _device_engines_lock:
+        e = _device_engines.get(device)
+        if e is None:
+            e = _device_engines[device] = Engine(device)
+        return e
 
 
 # ---- several samples in flight per GPU ---------------------------------------------------------

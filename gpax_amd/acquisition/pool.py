@@ -1,0 +1,466 @@
+"""
+Operators over a pool of candidates, the step after the acquisition values (gpax/acquisition/acquisition.py:22-35; the
+reference chooses by argmax, or by a softmax over the rewards, gpax/hypo.py:115-167, on the host): the softmax policy over
+a row of scores, its gradient, the weight that candidates gather over many rows, and the eviction that keeps a pool within
+a budget by that weight (include/gpx.h, csrc/choice.hip, csrc/pool.hip).
+
+Arguments are either all NumPy arrays, which are staged through the default engine's GPU and come back as NumPy arrays, or
+all torch tensors on one GPU, which are worked on in place on torch's current stream, without a copy and without waiting
+(import torch before the library is loaded, so that both use one HIP runtime; the first call on a GPU makes its context and
+must not be inside a graph capture).  No autograd graph is recorded: `choice_logprobs_grad` is the backward pass, and a
+tensor that requires grad is refused while gradients are enabled.
+
+Scores are (M,), (rows, M) or (pools, rows, M), of any strides, in float64, float32, bfloat16 or float16.  Sums,
+statistics and all real results but gradients are float64 for float64 scores and float32 for the others.  A candidate
+exists for a row if it lies below the row's length, its mask is true and its score is not -inf (as penalised acquisition
+values are); what is stored in other places is never used.
+"""
+import functools
+import math
+import sys
+from typing import NamedTuple, Optional, Sequence
+
+import numpy as np
+
+from .. import _lib
+
+MAX_TOP = 64
+MAX_PAYLOAD = 16
+_DTYPES = {"float64": 0, "float32": 1, "bfloat16": 2, "float16": 3}
+
+
+class ChoiceLogprobs(NamedTuple):
+    """Results of `choice_logprobs`; `stats` (the row's largest score and the log2 of its sum) is what
+    `choice_logprobs_grad` reads."""
+    logprobs: object
+    entropy: object
+    logsumexp: object
+    top_indices: object
+    top_logprobs: object
+    stats: object
+
+
+class PoolEviction(NamedTuple):
+    """Results of `pool_evict`."""
+    indices: object
+    lengths: object
+    weights: object
+    payload: tuple
+
+
+def _is_torch(a) -> bool:
+    return type(a).__module__.partition(".")[0] == "torch"
+
+
+@functools.lru_cache(maxsize=1)
+def _one_runtime() -> bool:
+    """Device addresses and streams of torch mean something to the library only if both run on one HIP runtime."""
+    _lib.load_library()
+    try:
+        with open("/proc/self/maps") as f:
+            found = {line.split(None, 5)[5].strip() for line in f if "libamdhip64.so" in line}
+    except OSError:
+        return True
+    return len(found) <= 1
+
+
+class _Device:
+    """Torch tensors on one GPU."""
+    host = False
+
+    def __init__(self, ref):
+        self.torch = sys.modules["torch"]
+        if not isinstance(ref, self.torch.Tensor) or not ref.is_cuda:
+            raise ValueError("torch tensors must be on a GPU; pass NumPy arrays for data on the host")
+        if not _one_runtime():
+            raise _lib.GpxError("libgpx and torch have loaded two HIP runtimes: import torch before gpax_amd's library is "
+                                "loaded (before the first engine)")
+        self.ref, self.device = ref, ref.device
+        self.engine = _lib.get_device_engine(ref.device.index)
+
+    def take(self, a, name: str, kinds: Sequence[str], contiguous: bool = False):
+        if not isinstance(a, self.torch.Tensor) or a.device != self.device:
+            raise ValueError(f"{name} must be a torch tensor on {self.device}, as the first argument is")
+        kind = str(a.dtype)[6:]
+        if kind not in kinds:
+            raise ValueError(f"{name} has dtype {kind}; expected {' or '.join(kinds)}")
+        if a.requires_grad and self.torch.is_grad_enabled():
+            raise ValueError(f"{name} requires grad, and no graph is recorded: detach it and call choice_logprobs_grad")
+        if a.is_conj() or a.is_neg():
+            a = a.resolve_neg()
+        return a.contiguous() if contiguous else a
+
+    def kind(self, a) -> str:
+        return str(a.dtype)[6:]
+
+    def strides(self, a):
+        return a.stride()
+
+    def new(self, shape, kind: str):
+        return self.ref.new_empty(shape, dtype=getattr(self.torch, kind), requires_grad=False)
+
+    def room(self, nbytes: int):
+        return self.new((nbytes,), "uint8") if nbytes else None
+
+    def run(self, inputs, outputs, fn, room=None) -> None:
+        stream = self.torch.cuda.current_stream(self.device).cuda_stream
+        with self.engine._pool_lock:
+            fn(self.engine, lambda a: 0 if a is None else a.data_ptr(), stream)
+
+
+class _Room(NamedTuple):
+    """Workspace of a host call: space in the scratch, nothing to copy."""
+    nbytes: int
+
+
+class _Host:
+    """NumPy arrays, staged through the default engine's scratch."""
+    host = True
+
+    def __init__(self, ref):
+        self.engine = _lib.get_engine()
+
+    def take(self, a, name: str, kinds: Sequence[str], contiguous: bool = False):
+        if _is_torch(a):
+            raise ValueError(f"{name} is a torch tensor and the first argument is not")
+        a = np.asarray(a)
+        if a.dtype.name not in kinds:
+            want = kinds[0]
+            if want == "bool" or a.dtype.kind not in "iuf" or (want == "int64" and a.dtype.kind == "f"):
+                raise ValueError(f"{name} has dtype {a.dtype.name}; expected {' or '.join(kinds)}")
+            a = a.astype(want)
+        return np.ascontiguousarray(a) if a.ndim else a.copy()
+
+    def kind(self, a) -> str:
+        return a.dtype.name
+
+    def strides(self, a):
+        return tuple(s // a.itemsize for s in a.strides)
+
+    def new(self, shape, kind: str):
+        return np.empty(shape, dtype=kind)
+
+    def room(self, nbytes: int):
+        return _Room(nbytes) if nbytes else None
+
+    def run(self, inputs, outputs, fn, room=None) -> None:
+        place, at = {}, 0
+        for a in (*inputs, *outputs, room):
+            if a is not None and id(a) not in place:
+                place[id(a)] = at
+                at += (a.nbytes + 255) // 256 * 256
+        with self.engine._pool_lock:
+            base = self.engine.scratch(at)
+            for a in inputs:
+                if a is not None:
+                    self.engine.upload(base + place[id(a)], a)
+            fn(self.engine, lambda a: 0 if a is None else base + place[id(a)], self.engine.stream())
+            for a in outputs:
+                if a is not None:
+                    self.engine.download(a, base + place[id(a)])
+
+
+def _space(a):
+    return _Device(a) if _is_torch(a) else _Host(a)
+
+
+def _broadcast_strides(shape, strides, to, name: str):
+    """Strides that read an array of `shape` as one of shape `to`."""
+    lead = len(to) - len(shape)
+    out = [0] * len(to)
+    for i, (n, s) in enumerate(zip(shape, strides)):
+        if lead + i < 0 or (n != 1 and n != to[lead + i]):
+            raise ValueError(f"{name} has shape {tuple(shape)}, which does not broadcast to {tuple(to)}")
+        out[lead + i] = 0 if n == 1 else s
+    return out
+
+
+def _padded(values, n: int):
+    return [0] * (n - len(values)) + list(values)
+
+
+class _Policy:
+    """Checked scores, mask, lengths and temperature of a call."""
+
+    def __init__(self, scores, temperature, mask, lengths):
+        self.space = space = _space(scores)
+        self.scores = x = space.take(scores, "scores", ("float64", "float32", "float16") if space.host else tuple(_DTYPES))
+        if not 1 <= x.ndim <= 3:
+            raise ValueError(f"scores have shape {tuple(x.shape)}; expected (M,), (rows, M) or (pools, rows, M)")
+        self.kind = space.kind(x)
+        self.acc = "float64" if self.kind == "float64" else "float32"
+        self.shape = shape = tuple(x.shape)
+        self.lead, self.M = shape[:-1], shape[-1]
+        p, r = _padded(self.lead, 2) if len(shape) == 3 else (1, shape[0] if len(shape) == 2 else 1)
+        self.pools, self.rows = p, r
+        if p * r > 1 << 25:
+            raise ValueError("more than 2^25 rows of scores")
+        if self.M > (1 << 31) - 1 - 65536:
+            raise ValueError("more than 2^31 - 65537 candidates")
+        self.mask = self.lengths = self.temps = None
+        self.mask_strides = self.lengths_strides = self.temps_strides = ()
+        if mask is not None:
+            self.mask = m = space.take(mask, "mask", ("bool", "uint8"))
+            self.mask_strides = _broadcast_strides(tuple(m.shape), space.strides(m), shape, "mask")
+        if lengths is not None:
+            self.lengths = n = space.take(lengths, "lengths", ("int64", "int32"))
+            self.lengths_strides = _broadcast_strides(tuple(n.shape), space.strides(n), self.lead, "lengths")
+        if isinstance(temperature, (int, float, np.number)):
+            self.temperature = float(temperature)
+            least = 2.3e-308 if self.acc == "float64" else 1.2e-38
+            if not (least <= self.temperature < math.inf) or (self.acc == "float32" and self.temperature > 3.4e38):
+                raise ValueError("the temperature must be positive and finite")
+        else:
+            self.temperature = 1.0
+            self.temps = t = space.take(temperature, "temperature", (self.acc,))
+            self.temps_strides = _broadcast_strides(tuple(t.shape), space.strides(t), self.lead, "temperature")
+            if space.host and not (np.all(t > 0) and np.all(np.isfinite(t))):
+                raise ValueError("the temperature must be positive and finite")
+
+    def inputs(self):
+        return self.scores, self.mask, self.lengths, self.temps
+
+    def struct(self, ptr) -> "_lib.PoolScores":
+        return _lib.PoolScores(
+            ptr(self.scores), self.pools, self.rows, self.M, tuple(_padded(self.space.strides(self.scores), 3)),
+            ptr(self.mask) if self.mask is not None else 0, tuple(_padded(self.mask_strides, 3)),
+            ptr(self.lengths) if self.lengths is not None else 0, tuple(_padded(self.lengths_strides, 2)),
+            ptr(self.temps) if self.temps is not None else 0, tuple(_padded(self.temps_strides, 2)),
+            self.temperature, _DTYPES[self.kind], int(self.lengths is not None and self.space.kind(self.lengths) == "int64"))
+
+    def choices(self, choices):
+        """(choices, number per row, shape of the log probabilities)"""
+        if choices is None:
+            return None, 0, self.lead + (0,)
+        if isinstance(choices, (int, np.integer)) and self.space.host:
+            choices = np.int64(choices)
+        c = self.space.take(choices, "choices", ("int64", "int32"), contiguous=True)
+        shape = tuple(c.shape)
+        if shape != self.lead and shape[:-1] != self.lead or len(shape) > len(self.lead) + 1:
+            raise ValueError(f"choices have shape {shape}; expected {self.lead} or {self.lead + ('C',)}")
+        if self.space.kind(c) == "int32":
+            c = c.astype(np.int64) if self.space.host else c.long()
+        if self.space.host and c.size and (c.min() < -1 or c.max() >= self.M):
+            raise ValueError(f"choices must lie in 0 .. {self.M - 1}, or be -1")
+        n = 1 if len(shape) == len(self.lead) else shape[-1]
+        return c, n, shape
+
+
+@functools.lru_cache(maxsize=4096)
+def _choice_workspace(pools, rows, M, dtype, top) -> int:
+    return _lib.load_library().gpx_choice_workspace(pools, rows, M, dtype, top)
+
+
+@functools.lru_cache(maxsize=4096)
+def _weights_workspace(pools, rows, M, dtype) -> int:
+    return _lib.load_library().gpx_pool_weights_workspace(pools, rows, M, dtype)
+
+
+def choice_logprobs(scores, choices=None, *, temperature=1.0, mask=None, lengths=None, top: int = 0) -> ChoiceLogprobs:
+    """Softmax policy p_j = exp(x_j / T) / sum_i exp(x_i / T) over every row of scores, in one pass over them.
+
+    Args:
+        scores: (M,), (rows, M) or (pools, rows, M)
+        choices: the candidates whose log probabilities are wanted, shape scores.shape[:-1] (one a row) or
+            scores.shape[:-1] + (C,); -1 is a filler (log probability 0), a candidate that does not exist has -inf
+            (a number outside the pool: ValueError for NumPy arrays, NaN for tensors)
+        temperature: T, a number or an array broadcast to the rows (of the accumulator's type)
+        mask: which candidates may be chosen, bool or uint8, broadcast to the scores
+        lengths: how many candidates each row has, int64 or int32, broadcast to the rows (clamped to 0 .. M)
+        top: number of best alternatives to return, at most 64
+
+    Returns:
+        ChoiceLogprobs: logprobs (as choices), entropy and logsumexp (one a row), top_indices and top_logprobs (rows, top):
+        score descending, equal scores by index, -1 and -inf where fewer exist; a row in which nothing exists has entropy 0
+        and logsumexp -inf; a row with a NaN or +inf among what exists is NaN (NaN scores are never alternatives)
+    """
+    pol = _Policy(scores, temperature, mask, lengths)
+    top = int(top)
+    if not 0 <= top <= MAX_TOP:
+        raise ValueError(f"top is {top}; expected 0 .. {MAX_TOP}")
+    c, n, lp_shape = pol.choices(choices)
+    sp = pol.space
+    logprobs, entropy, lse = sp.new(lp_shape, pol.acc), sp.new(pol.lead, pol.acc), sp.new(pol.lead, pol.acc)
+    stats = sp.new(pol.lead + (2,), pol.acc)
+    top_i, top_lp = sp.new(pol.lead + (top,), "int64"), sp.new(pol.lead + (top,), pol.acc)
+    nbytes = _choice_workspace(pol.pools, pol.rows, pol.M, _DTYPES[pol.kind], top)
+    ws = sp.room(nbytes)
+
+    def call(engine, ptr, stream):
+        engine.choice_logprobs(pol.struct(ptr), ptr(c), n, top, ptr(logprobs), ptr(entropy), ptr(lse), ptr(stats), ptr(top_i),
+                               ptr(top_lp), ptr(ws), nbytes, stream)
+
+    sp.run((*pol.inputs(), c), (logprobs, entropy, lse, stats, top_i, top_lp), call, ws)
+    return ChoiceLogprobs(logprobs, entropy, lse, top_i, top_lp, stats)
+
+
+def choice_logprobs_grad(scores, forward: ChoiceLogprobs, choices=None, *, grad_logprobs=None, grad_entropy=None,
+                         grad_logsumexp=None, grad_top_logprobs=None, temperature=1.0, mask=None, lengths=None):
+    """Gradient with respect to the scores of sum(grad_logprobs * logprobs) + sum(grad_entropy * entropy) +
+    sum(grad_logsumexp * logsumexp) + sum(grad_top_logprobs * top_logprobs), the selection of alternatives held fixed.
+
+    Args:
+        scores, choices, temperature, mask, lengths: as in the forward call
+        forward: what the forward call returned
+        grad_logprobs, grad_entropy, grad_logsumexp, grad_top_logprobs: gradients of the results, of their shapes and of the
+            accumulator's type; None: zero
+
+    Returns:
+        the gradient, contiguous, of the scores' shape and type (computed in the accumulator's type, rounded once).  Fillers
+        and choices that do not exist have none; a choice named twice counts twice, in the order of the choices.
+    """
+    pol = _Policy(scores, temperature, mask, lengths)
+    sp, acc = pol.space, pol.acc
+    c, n, lp_shape = pol.choices(choices)
+
+    def result(a, name, shape, kinds):
+        a = sp.take(a, name, kinds, contiguous=True)
+        if tuple(a.shape) != tuple(shape):
+            raise ValueError(f"{name} has shape {tuple(a.shape)}; expected {tuple(shape)}")
+        return a
+
+    if not isinstance(forward, ChoiceLogprobs):
+        raise ValueError("forward must be what choice_logprobs returned")
+    stats = result(forward.stats, "forward.stats", pol.lead + (2,), (acc,))
+    logprobs = entropy = top_i = None
+    g_lp = g_h = g_lse = g_top = None
+    top = 0
+    if grad_logprobs is not None:
+        if c is None:
+            raise ValueError("grad_logprobs needs the choices of the forward call")
+        g_lp = result(grad_logprobs, "grad_logprobs", lp_shape, (acc,))
+        logprobs = result(forward.logprobs, "forward.logprobs", lp_shape, (acc,))
+    if grad_entropy is not None:
+        g_h = result(grad_entropy, "grad_entropy", pol.lead, (acc,))
+        entropy = result(forward.entropy, "forward.entropy", pol.lead, (acc,))
+    if grad_logsumexp is not None:
+        g_lse = result(grad_logsumexp, "grad_logsumexp", pol.lead, (acc,))
+    if grad_top_logprobs is not None:
+        top = int(forward.top_indices.shape[-1])
+        top_i = result(forward.top_indices, "forward.top_indices", pol.lead + (top,), ("int64",))
+        g_top = result(grad_top_logprobs, "grad_top_logprobs", pol.lead + (top,), (acc,))
+    grad = sp.new(pol.shape, pol.kind)
+
+    def call(engine, ptr, stream):
+        engine.choice_logprobs_grad(pol.struct(ptr), ptr(c), n, ptr(logprobs), ptr(g_lp), top, ptr(top_i), ptr(g_top),
+                                    ptr(entropy), ptr(stats), ptr(g_h), ptr(g_lse), ptr(grad), stream)
+
+    sp.run((*pol.inputs(), c, logprobs, g_lp, top_i, g_top, entropy, stats, g_h, g_lse), (grad,), call)
+    return grad
+
+
+def pool_weights(scores, weights=None, *, decay: float = 1.0, row_weights=None, temperature=1.0, mask=None, lengths=None,
+                 out=None):
+    """The weight each candidate has gathered: decay * weights + the sum of its probability p over the rows.  Over posterior
+    draws, divided by their number, it is the (tempered) probability of being the best candidate.
+
+    Args:
+        scores: (M,), (rows, M) or (pools, rows, M)
+        weights: weights gathered before, (M,) or (pools, M), of the accumulator's type; None: zeros
+        decay: factor on them, finite and not negative
+        row_weights: factor of each row, of the accumulator's type, shape scores.shape[:-1]; a row of weight 0 is not read
+        temperature, mask, lengths: as for choice_logprobs
+        out: array for the result (may be `weights`)
+
+    Returns:
+        the new weights, (M,) or (pools, M).  A row in which nothing exists adds nothing; a NaN row makes what exists in it
+        NaN.  The sums have a fixed order: the same call gives the same bits.
+    """
+    pol = _Policy(scores, temperature, mask, lengths)
+    sp = pol.space
+    decay = float(decay)
+    if not 0.0 <= decay < math.inf:
+        raise ValueError("the decay must be finite and not negative")
+    if pol.pools > 65535:
+        raise ValueError("more than 65535 pools")
+    shape = (pol.pools, pol.M) if len(pol.shape) == 3 else (pol.M,)
+    w = u = None
+    if weights is not None:
+        w = sp.take(weights, "weights", (pol.acc,), contiguous=True)
+        if tuple(w.shape) != shape:
+            raise ValueError(f"weights have shape {tuple(w.shape)}; expected {shape}")
+    if row_weights is not None:
+        u = sp.take(row_weights, "row_weights", (pol.acc,), contiguous=True)
+        if tuple(u.shape) != pol.lead:
+            raise ValueError(f"row_weights have shape {tuple(u.shape)}; expected {pol.lead}")
+    if out is None:
+        res = sp.new(shape, pol.acc)
+    else:
+        res = sp.take(out, "out", (pol.acc,)) if not sp.host else out
+        ok = tuple(res.shape) == shape and (res.is_contiguous() if not sp.host else
+                                            res.flags.c_contiguous and res.flags.writeable and res.dtype.name == pol.acc)
+        if not ok:
+            raise ValueError(f"out must be contiguous, of shape {shape} and of type {pol.acc}")
+    nbytes = _weights_workspace(pol.pools, pol.rows, pol.M, _DTYPES[pol.kind])
+    ws = sp.room(nbytes)
+
+    def call(engine, ptr, stream):
+        engine.pool_weights(pol.struct(ptr), ptr(u), ptr(w), decay, ptr(res), ptr(ws), nbytes, stream)
+
+    sp.run((*pol.inputs(), w, u), (res,), call, ws)
+    return res
+
+
+def pool_evict(weights, budget: int, payload: Sequence = (), *, first: int = 0, recent: int = 0,
+               lengths: Optional[object] = None) -> PoolEviction:
+    """Cut a pool, or every one of several, to at most `budget` candidates: the `first` first and the `recent` last ones
+    stay, of the others those of largest weight (equal weights: the lower index; NaN: the smallest).
+
+    Args:
+        weights: gathered weights, (M,) or (pools, M), float64 or float32
+        budget: how many candidates stay at most, positive
+        payload: at most 16 arrays of shape weights.shape + (...) whose rows move along (the points themselves)
+        first, recent: how many of the first and of the last stay whatever their weight; together at most the budget
+        lengths: how many candidates each pool has, int64 or int32, broadcast to (pools,); clamped to 0 .. M
+
+    Returns:
+        PoolEviction: indices (budget, ascending), lengths, weights and payload of what stayed, in the order it had; behind
+        the last one index -1 and zeros.  Nothing is changed in place.
+    """
+    sp = _space(weights)
+    w = sp.take(weights, "weights", ("float64", "float32"), contiguous=True)
+    if not 1 <= w.ndim <= 2:
+        raise ValueError(f"weights have shape {tuple(w.shape)}; expected (M,) or (pools, M)")
+    lead, M = tuple(w.shape[:-1]), int(w.shape[-1])
+    pools = lead[0] if lead else 1
+    budget, first, recent = int(budget), int(first), int(recent)
+    if not 1 <= budget <= (1 << 31) - 1:
+        raise ValueError(f"the budget is {budget}; expected a positive number")
+    if first < 0 or recent < 0 or first + recent > budget:
+        raise ValueError(f"first = {first} and recent = {recent} must not be negative, and together at most the budget {budget}")
+    if pools > (1 << 19) - 1 or M > (1 << 31) - 1 - 65536:
+        raise ValueError("more than 2^19 - 1 pools, or 2^31 - 65537 candidates")
+    n, n_stride, n64 = None, 0, False
+    if lengths is not None:
+        n = sp.take(lengths, "lengths", ("int64", "int32"))
+        stride = _broadcast_strides(tuple(n.shape), sp.strides(n), lead, "lengths")
+        n_stride, n64 = (stride[0] if stride else 0), sp.kind(n) == "int64"
+    payload = tuple(payload)
+    if len(payload) > MAX_PAYLOAD:
+        raise ValueError(f"{len(payload)} payload arrays; at most {MAX_PAYLOAD}")
+    moved, moved_out, row_bytes = [], [], []
+    for i, a in enumerate(payload):
+        kinds = _PAYLOAD if not sp.host else (np.asarray(a).dtype.name,)
+        a = sp.take(a, f"payload[{i}]", kinds, contiguous=True)
+        if sp.host and a.dtype.kind not in "biufc":
+            raise ValueError(f"payload[{i}] has dtype {a.dtype.name}; expected numbers")
+        if tuple(a.shape[: len(lead) + 1]) != lead + (M,):
+            raise ValueError(f"payload[{i}] has shape {tuple(a.shape)}; expected {lead + (M,)} + (...)")
+        moved.append(a)
+        moved_out.append(sp.new(lead + (budget,) + tuple(a.shape[len(lead) + 1:]), sp.kind(a)))
+        size = a.itemsize if sp.host else a.element_size()
+        row_bytes.append(math.prod(a.shape[len(lead) + 1:]) * size)
+        if row_bytes[-1] > (1 << 31) - 1:
+            raise ValueError(f"payload[{i}] has rows of 2 GiB or more")
+    indices, left, w_out = sp.new(lead + (budget,), "int64"), sp.new(lead, "int64"), sp.new(lead + (budget,), sp.kind(w))
+
+    def call(engine, ptr, stream):
+        engine.pool_evict(_DTYPES[sp.kind(w)], pools, M, ptr(w), ptr(n), n64, n_stride, budget, first, recent, ptr(indices),
+                          ptr(left), ptr(w_out), [ptr(a) for a in moved], [ptr(a) for a in moved_out], row_bytes, stream)
+
+    sp.run((w, n, *moved), (indices, left, w_out, *moved_out), call)
+    return PoolEviction(indices, left, w_out, tuple(moved_out))
+
+
+_PAYLOAD = ("float64", "float32", "bfloat16", "float16", "float8_e4m3fn", "float8_e5m2", "int64", "int32", "int16", "int8",
+            "uint8", "bool", "complex64", "complex128")

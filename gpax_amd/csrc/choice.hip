@@ -1,0 +1,564 @@
+// choice.hip — the softmax policy over a pool of candidates: log probabilities of given choices, entropy, log of the sum of
+// exponentials and the best alternatives of every row in ONE pass over the scores, and the gradient of all of them.
+//
+// Bound by memory for large pools (a score is read once; 3 - 4 fused operations and one exponential each) and by latency for
+// small ones.  A row is worked on by 1, 4 or 16 waves of one workgroup, or by several workgroups whose partial results a
+// second launch joins: as many waves as it takes to occupy the chip, no more (choice_plan).
+//
+// Alternatives: every wave keeps the best 64 candidates it has met, one per lane, sorted by (score descending, index
+// ascending).  The k-th of them is a threshold that few later candidates pass: a step whose largest score does not is left
+// with one comparison.  The few that do are inserted one by one (a ballot gives the position, a shift by one lane makes
+// room); many at once are sorted across the lanes and merged.  Lists of waves and workgroups are merged the same way, so
+// the order in which they arrive decides nothing: equal scores are told apart by their index.
+#include "pool.h"
+
+using namespace gpx;
+
+namespace {
+
+constexpr int TOP_MAX = 64;    // alternatives per row: one per lane of a wave
+constexpr int INSERT_MAX = 10; // more than this many newcomers in one vector: sort and merge instead of inserting one by one
+
+struct ChoiceArgs {
+  PoolScores sc;
+  const int64_t* choices; // rows x C, -1 = filler
+  int C;
+  int top;
+  int splits; // workgroups per row
+  void *logprobs, *entropy, *lse, *stats, *top_logprobs;
+  int64_t* top_indices;
+  void* ws;
+};
+
+// A partial result in the workspace: statistics and the list, of one split of one row
+template <typename A>
+struct Partial {
+  A m, s, t, pad;
+};
+inline int64_t partial_bytes(int acc_size, int top) { return 4 * acc_size + round_up64((int64_t)top * (acc_size + 4), 16); }
+
+__device__ __forceinline__ float read_lane(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
+__device__ __forceinline__ uint32_t read_lane(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
+__device__ __forceinline__ double read_lane(double v, int l) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l));
+}
+
+template <typename A>
+__device__ __forceinline__ bool before(A k1, uint32_t i1, A k2, uint32_t i2) {
+  return k1 > k2 || (k1 == k2 && i1 < i2);
+}
+
+template <typename A>
+struct TopList {
+  A key;        // lane l: the l-th best; -inf where there is none
+  uint32_t idx; // ... and its index; all ones where there is none
+  A thr_key;    // the k-th (uniform)
+  uint32_t thr_idx;
+  int k;
+
+  __device__ __forceinline__ void init(int k_) {
+    key = thr_key = neg_inf<A>();
+    idx = thr_idx = 0xffffffffu;
+    k = k_;
+  }
+  __device__ __forceinline__ void rethreshold() {
+    thr_key = read_lane(key, k - 1);
+    thr_idx = read_lane(idx, k - 1);
+  }
+  static __device__ __forceinline__ void exchange(A& kk, uint32_t& ii, int stride, bool keep_first) {
+    const A ok = __shfl_xor(kk, stride);
+    const uint32_t oi = __shfl_xor(ii, stride);
+    if (before(kk, ii, ok, oi) != keep_first) {
+      kk = ok;
+      ii = oi;
+    }
+  }
+  static __device__ __forceinline__ void sort(A& kk, uint32_t& ii, int lane) {
+#pragma unroll 1
+    for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll 1
+      for (int stride = size >> 1; stride > 0; stride >>= 1) exchange(kk, ii, stride, ((lane & stride) == 0) == ((lane & size) == 0));
+  }
+  // one sorted list into this one: the better of (mine, other reversed) lane by lane holds the best 64 of both as a bitonic
+  // sequence, six exchanges sort it
+  __device__ __forceinline__ void merge_sorted(A ck, uint32_t ci, int lane) {
+    const A rk = __shfl(ck, 63 - lane);
+    const uint32_t ri = __shfl(ci, 63 - lane);
+    if (before(rk, ri, key, idx)) {
+      key = rk;
+      idx = ri;
+    }
+#pragma unroll 1
+    for (int stride = 32; stride > 0; stride >>= 1) exchange(key, idx, stride, (lane & stride) == 0);
+    rethreshold();
+  }
+  __device__ __forceinline__ void consume(A x, uint32_t j, int lane) {
+    const bool pass = x > neg_inf<A>() && before(x, j, thr_key, thr_idx); // NaN never passes
+    uint64_t in = __ballot(pass);
+    if (in == 0) return;
+    if (__popcll(in) > INSERT_MAX) {
+      A ck = pass ? x : neg_inf<A>();
+      uint32_t ci = pass ? j : 0xffffffffu;
+      sort(ck, ci, lane);
+      merge_sorted(ck, ci, lane);
+      return;
+    }
+    while (in) {
+      const int l = __ffsll((unsigned long long)in) - 1;
+      in &= in - 1;
+      const A nk = read_lane(x, l);
+      const uint32_t ni = read_lane(j, l);
+      const bool ahead = before(key, idx, nk, ni);
+      const int at = __popcll(__ballot(ahead));
+      const A pk = __shfl_up(key, 1);
+      const uint32_t pi = __shfl_up(idx, 1);
+      if (!ahead) {
+        key = lane == at ? nk : pk;
+        idx = lane == at ? ni : pi;
+      }
+    }
+    rethreshold();
+  }
+  // a list that is sorted already
+  __device__ __forceinline__ void consume_sorted(A ck, uint32_t ci, int lane) {
+    if (__ballot(before(ck, ci, thr_key, thr_idx)) == 0) return;
+    merge_sorted(ck, ci, lane);
+  }
+};
+
+// What a row's statistics are turned into, by a team of `size` threads of which this one is `at`; the list by its wave.
+template <typename T>
+__device__ __forceinline__ void finish_row(const ChoiceArgs& a, int64_t row, int64_t b, int64_t r, const Stats<typename Acc<T>::type>& st, int at,
+                                           int size) {
+  typedef typename Acc<T>::type A;
+  const A log2s = log2_acc(st.s), log_s = ln2<A>() * log2s, T_row = row_temperature<A>(a.sc, b, r);
+  if (at == 0) {
+    if (a.entropy) static_cast<A*>(a.entropy)[row] = stats_entropy(st, log2s);
+    if (a.lse) static_cast<A*>(a.lse)[row] = st.m / T_row + log_s;
+    if (a.stats) {
+      static_cast<A*>(a.stats)[2 * row] = st.m;
+      static_cast<A*>(a.stats)[2 * row + 1] = log2s;
+    }
+  }
+  if (a.C > 0) {
+    const Row<T> v = row_view<T>(a.sc, b, r);
+    for (int q = at; q < a.C; q += size) {
+      const int64_t j = a.choices[row * a.C + q];
+      A lp = (A)0; // a filler
+      if (j >= a.sc.M || j < -1) {
+        lp = (A)NAN; // no candidate of this pool: never read
+      } else if (j >= 0) {
+        const A x = row_at(v, (int)j);
+        lp = x == neg_inf<A>() ? x : (x - st.m) / T_row - log_s; // not through powers of two: a lowest score overflows there
+      }
+      static_cast<A*>(a.logprobs)[row * a.C + q] = lp;
+    }
+  }
+}
+template <typename A>
+__device__ __forceinline__ void finish_top(const ChoiceArgs& a, int64_t row, int64_t b, int64_t r, const Stats<A>& st, const TopList<A>& list, int lane) {
+  if (lane >= a.top) return;
+  const bool there = list.idx != 0xffffffffu;
+  a.top_indices[row * a.top + lane] = there ? (int64_t)list.idx : -1;
+  static_cast<A*>(a.top_logprobs)[row * a.top + lane] =
+      there ? (list.key - st.m) / row_temperature<A>(a.sc, b, r) - ln2<A>() * log2_acc(st.s) : neg_inf<A>();
+}
+
+// Joins the statistics and lists of the W waves of a workgroup: log2 W rounds, each wave with the one `half` above it.
+template <typename A, int W, bool TOP>
+__device__ __forceinline__ void join_waves(Stats<A>& st, TopList<A>& list, A c, int wave, int lane) {
+  __shared__ Stats<A> sh_st[W];
+  __shared__ A sh_key[TOP ? W : 1][64];
+  __shared__ uint32_t sh_idx[TOP ? W : 1][64];
+#pragma unroll 1
+  for (int half = W / 2; half > 0; half >>= 1) {
+    if (wave >= half && wave < 2 * half) {
+      if (lane == 0) sh_st[wave] = st;
+      if (TOP) {
+        sh_key[wave][lane] = list.key;
+        sh_idx[wave][lane] = list.idx;
+      }
+    }
+    __syncthreads();
+    if (wave < half) {
+      st = stats_join(st, sh_st[wave + half], c);
+      if (TOP) list.consume_sorted(sh_key[wave + half][lane], sh_idx[wave + half][lane], lane);
+    }
+  }
+}
+
+template <typename T, int WAVES, bool TOP>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void choice_rows_kernel(ChoiceArgs a) {
+  typedef typename Acc<T>::type A;
+  constexpr int VEC = VecOf<T>::value;
+  constexpr int U = sizeof(T) == 8 ? 8 : 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+  if (row >= a.sc.rows) return; // WAVES == 1: whole waves, and no barrier below
+  const int64_t b = (uint32_t)row / (uint32_t)a.sc.R, r = row - b * a.sc.R; // at most 2^25 rows
+  const A c = temperature_scale(row_temperature<A>(a.sc, b, r));
+  const Row<T> v = row_view<T>(a.sc, b, r);
+  Stats<A> st = stats_empty<A>();
+  TopList<A> list;
+  if (TOP) list.init(a.top);
+  const int64_t step = (int64_t)64 * VEC * U;
+  const int64_t first = WAVES == 1 ? 0 : ((int64_t)blockIdx.y * WAVES + wave) * step;
+  const int64_t stride = WAVES == 1 ? step : (int64_t)a.splits * WAVES * step;
+  for (int64_t j0 = first; j0 < v.n; j0 += stride) {
+    A x[U * VEC];
+    load_step<T, VEC, U>(v, j0, 64 * VEC, lane * VEC, x);
+    A cm = x[0];
+#pragma unroll
+    for (int e = 1; e < U * VEC; ++e) cm = fmax(cm, x[e]);
+    stats_add<A, U * VEC>(st, x, cm, c);
+    if (TOP) {
+      // strictly above: a score equal to the k-th loses to it, whose index is lower (steps are taken in order)
+      if (__ballot(cm > list.thr_key) != 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) list.consume(x[u * VEC + e], (uint32_t)(j0 + u * 64 * VEC + lane * VEC + e), lane);
+      }
+    }
+  }
+  st = stats_wave(st, c);
+  if constexpr (WAVES > 1) join_waves<A, WAVES, TOP>(st, list, c, wave, lane);
+  if (WAVES == 1 || a.splits == 1) {
+    if (WAVES == 1) {
+      finish_row<T>(a, row, b, r, st, lane, 64);
+    } else {
+      __shared__ Stats<A> sh;
+      if (threadIdx.x == 0) sh = st;
+      __syncthreads();
+      finish_row<T>(a, row, b, r, sh, threadIdx.x, WAVES * 64);
+    }
+    if (TOP && (WAVES == 1 || wave == 0)) finish_top(a, row, b, r, st, list, lane);
+  } else if (wave == 0) {
+    char* at = static_cast<char*>(a.ws) + (row * a.splits + blockIdx.y) * (4 * (int64_t)sizeof(A) + (((int64_t)a.top * (sizeof(A) + 4) + 15) / 16 * 16));
+    if (lane == 0) *reinterpret_cast<Partial<A>*>(at) = Partial<A>{st.m, st.s, st.t, (A)0};
+    if (TOP && lane < a.top) {
+      reinterpret_cast<A*>(at + 4 * sizeof(A))[lane] = list.key;
+      reinterpret_cast<uint32_t*>(at + 4 * sizeof(A) + a.top * sizeof(A))[lane] = list.idx;
+    }
+  }
+}
+
+// One workgroup per row: the partial results of its splits, dealt to the waves.
+template <typename T, int WAVES, bool TOP>
+__global__ __launch_bounds__(WAVES * 64) void choice_join_kernel(ChoiceArgs a) {
+  typedef typename Acc<T>::type A;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = blockIdx.x;
+  const int64_t b = (uint32_t)row / (uint32_t)a.sc.R, r = row - b * a.sc.R; // at most 2^25 rows
+  const A c = temperature_scale(row_temperature<A>(a.sc, b, r));
+  const int64_t bytes = 4 * (int64_t)sizeof(A) + (((int64_t)a.top * (sizeof(A) + 4) + 15) / 16 * 16);
+  const char* base = static_cast<const char*>(a.ws) + row * a.splits * bytes;
+  Stats<A> st = stats_empty<A>();
+  TopList<A> list;
+  if (TOP) list.init(a.top);
+  for (int s = wave; s < a.splits; s += WAVES) {
+    const Partial<A> p = *reinterpret_cast<const Partial<A>*>(base + s * bytes);
+    st = stats_join(st, Stats<A>{p.m, p.s, p.t}, c);
+    if (TOP) {
+      A k = neg_inf<A>();
+      uint32_t i = 0xffffffffu;
+      if (lane < a.top) {
+        k = reinterpret_cast<const A*>(base + s * bytes + 4 * sizeof(A))[lane];
+        i = reinterpret_cast<const uint32_t*>(base + s * bytes + 4 * sizeof(A) + a.top * sizeof(A))[lane];
+      }
+      list.consume_sorted(k, i, lane);
+    }
+  }
+  join_waves<A, WAVES, TOP>(st, list, c, wave, lane);
+  __shared__ Stats<A> sh;
+  if (threadIdx.x == 0) sh = st;
+  __syncthreads();
+  finish_row<T>(a, row, b, r, sh, threadIdx.x, WAVES * 64);
+  if (TOP && wave == 0) finish_top(a, row, b, r, st, list, lane);
+}
+
+// Gradient with respect to the scores of  sum g_lp log p(choice) + g_h entropy + g_lse lse + sum g_top log p(alternative):
+//   d / d z_j = p_j (g_lse - G - g_h (log p_j + entropy)) + sum over the choices and alternatives that are j of their g,
+// G = the sum of all g_lp and g_top that count (a filler, or a choice that may not be made, has no gradient), / T.
+// One wave per stretch of one row: elementwise given the row's statistics, so a score is read and a gradient written once.
+// The choices that fall into a stretch are found by a ballot and added in their order by the lane that holds the candidate:
+// the same choice twice gives the same bits every time.
+struct GradArgs {
+  PoolScores sc;
+  const int64_t* choices;
+  int C;
+  const void *logprobs, *g_logprobs;
+  const int64_t* top_indices;
+  int top;
+  const void *g_top, *entropy, *stats, *g_entropy, *g_lse;
+  void* grad; // rows x M, contiguous
+  int stretches;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void choice_grad_kernel(GradArgs a) {
+  typedef typename Acc<T>::type A;
+  constexpr int VEC = VecOf<T>::value;
+  constexpr int U = sizeof(T) == 8 ? 4 : 2;
+  constexpr int E = VEC * U;
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = unit / a.stretches;
+  if (row >= a.sc.rows) return;
+  const int64_t j0 = (unit - row * a.stretches) * (64 * E);
+  const int64_t b = (uint32_t)row / (uint32_t)a.sc.R, r = row - b * a.sc.R; // at most 2^25 rows
+  const Row<T> v = row_view<T>(a.sc, b, r);
+  A x[E];
+  load_step<T, VEC, U>(v, j0, 64 * VEC, lane * VEC, x);
+  const A Tm = row_temperature<A>(a.sc, b, r);
+  const A c = temperature_scale(Tm), inv_T = (A)1 / Tm;
+  const A m = static_cast<const A*>(a.stats)[2 * row], log2s = static_cast<const A*>(a.stats)[2 * row + 1];
+  const A h = a.g_entropy ? static_cast<const A*>(a.entropy)[row] : (A)0;
+  const A gh = a.g_entropy ? static_cast<const A*>(a.g_entropy)[row] : (A)0;
+  A add[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) add[e] = (A)0;
+  A G = (A)0;
+  auto gather = [&](const int64_t* idx, const A* g, const A* lp, int n) {
+    for (int q0 = 0; q0 < n; q0 += 64) {
+      const int q = q0 + lane;
+      int64_t j = -1;
+      A gq = (A)0;
+      if (q < n) {
+        j = idx[q];
+        gq = g[q];
+        if (j < 0 || j >= a.sc.M || (lp && lp[q] == neg_inf<A>())) {
+          j = -1;
+          gq = (A)0;
+        }
+      }
+      G += gq;
+      const bool here = j >= j0 && j < j0 + 64 * E;
+      for (uint64_t in = __ballot(here); in; in &= in - 1) {
+        const int l = __ffsll((unsigned long long)in) - 1;
+        const int off = __builtin_amdgcn_readlane((int)(j - j0), l);
+        const A gv = read_lane(gq, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (off == (e / VEC) * 64 * VEC + lane * VEC + e % VEC) add[e] += gv;
+      }
+    }
+  };
+  if (a.g_logprobs)
+    gather(a.choices + row * a.C, static_cast<const A*>(a.g_logprobs) + row * a.C, static_cast<const A*>(a.logprobs) + row * a.C, a.C);
+  if (a.g_top) gather(a.top_indices + row * a.top, static_cast<const A*>(a.g_top) + row * a.top, nullptr, a.top);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) G += __shfl_xor(G, o);
+  const A base = (a.g_lse ? static_cast<const A*>(a.g_lse)[row] : (A)0) - G;
+  T* out = static_cast<T*>(a.grad) + row * a.sc.M;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    Pack<T, VEC> o;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const A xe = x[u * VEC + e];
+      const A w = (xe - m) * c - log2s;
+      const A g = (exp2_acc(w) * (base - gh * (ln2<A>() * not_below_low(w) + h)) + add[u * VEC + e]) * inv_T;
+      from_acc(xe == neg_inf<A>() ? (A)0 : g, o.v[e]);
+    }
+    const int64_t j = j0 + u * 64 * VEC + lane * VEC;
+    if (j + VEC <= a.sc.M) {
+      *reinterpret_cast<Pack<T, VEC>*>(out + j) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (j + e < a.sc.M) out[j + e] = o.v[e];
+    }
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------
+
+// Waves per row (1, 4 or 16) and workgroups per row.  Enough waves to occupy the chip (TARGET), but none with less than a
+// step to do: a row shorter than that is one wave's, however few rows there are.
+struct ChoicePlan {
+  int waves, splits;
+};
+ChoicePlan choice_plan(int64_t rows, int64_t M, int dtype) {
+  constexpr int64_t TARGET = 4096;
+  const int64_t step = 64 * (dtype == GPX_DTYPE_F64 ? 16 : dtype == GPX_DTYPE_F32 ? 16 : 32);
+  const int64_t steps = (M + step - 1) / step;
+  int64_t want = rows > 0 ? (TARGET + rows - 1) / rows : 1;
+  if (want > steps) want = steps;
+  if (want <= 1) return ChoicePlan{1, 1};
+  if (want <= 4) return ChoicePlan{4, 1};
+  if (want <= 16) return ChoicePlan{16, 1};
+  int64_t splits = (want + 3) / 4;
+  if (splits > 64) splits = 64;
+  return ChoicePlan{4, (int)splits};
+}
+
+template <typename T, bool TOP>
+void choice_launch(const ChoiceArgs& a, ChoicePlan p, hipStream_t st) {
+  const unsigned rows = (unsigned)a.sc.rows;
+  if (p.waves == 1) {
+    hipLaunchKernelGGL((choice_rows_kernel<T, 1, TOP>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
+  } else if (p.waves == 16) {
+    hipLaunchKernelGGL((choice_rows_kernel<T, 16, TOP>), dim3(rows), dim3(1024), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((choice_rows_kernel<T, 4, TOP>), dim3(rows, p.splits), dim3(256), 0, st, a);
+    if (p.splits > 1) hipLaunchKernelGGL((choice_join_kernel<T, 16, TOP>), dim3(rows), dim3(1024), 0, st, a);
+  }
+}
+template <typename T>
+void choice_launch(const ChoiceArgs& a, ChoicePlan p, hipStream_t st) {
+  if (a.top > 0)
+    choice_launch<T, true>(a, p, st);
+  else
+    choice_launch<T, false>(a, p, st);
+}
+void choice_launch(int dtype, const ChoiceArgs& a, ChoicePlan p, hipStream_t st) {
+  switch (dtype) {
+    case GPX_DTYPE_F64: return choice_launch<double>(a, p, st);
+    case GPX_DTYPE_F32: return choice_launch<float>(a, p, st);
+    case GPX_DTYPE_BF16: return choice_launch<bf16_t>(a, p, st);
+    default: return choice_launch<f16_t>(a, p, st);
+  }
+}
+int acc_size(int dtype) { return dtype == GPX_DTYPE_F64 ? 8 : 4; }
+int64_t choice_workspace(int64_t rows, int64_t M, int dtype, int top) {
+  const ChoicePlan p = choice_plan(rows, M, dtype);
+  return p.splits == 1 ? 0 : rows * p.splits * partial_bytes(acc_size(dtype), top);
+}
+
+} // namespace
+
+namespace gpx {
+
+int pool_scores_view(gpx_ctx* ctx, const gpx_scores* x, PoolScores* out, const char* what) {
+  auto no = [&](const char* why) { return bad_arg(ctx, (std::string(what) + ": " + why).c_str()); };
+  if (!x) return no("null scores");
+  if (x->dtype < GPX_DTYPE_F64 || x->dtype > GPX_DTYPE_F16) return no("dtype");
+  if (x->pools < 0 || x->rows < 0 || x->candidates < 0) return no("negative size");
+  if (x->candidates > INT32_MAX - 65536) return no("more than 2^31 - 65536 candidates");
+  if (x->rows > 0 && x->pools > (int64_t)(1 << 25) / x->rows) return no("more than 2^25 rows");
+  if (x->pools * x->rows > 0 && x->candidates > 0 && !x->d_scores) return no("null scores");
+  if (!x->d_temperatures && !(x->temperature > 0 && x->temperature < INFINITY)) return no("the temperature must be positive and finite");
+  out->x = x->d_scores;
+  out->mask = x->d_mask;
+  out->lengths = x->d_lengths;
+  out->temps = x->d_temperatures;
+  out->xb = x->scores_stride[0];
+  out->xr = x->scores_stride[1];
+  out->xc = x->scores_stride[2];
+  out->mb = x->mask_stride[0];
+  out->mr = x->mask_stride[1];
+  out->mc = x->mask_stride[2];
+  out->lb = x->lengths_stride[0];
+  out->lr = x->lengths_stride[1];
+  out->tb = x->temperatures_stride[0];
+  out->tr = x->temperatures_stride[1];
+  out->R = x->rows;
+  out->rows = x->pools * x->rows;
+  out->M = (int)x->candidates;
+  out->len64 = x->lengths_64;
+  out->temperature = x->temperature;
+  return 0;
+}
+
+int64_t row_stats_workspace(int64_t rows, int64_t M, int dtype) { return choice_workspace(rows, M, dtype, 0); }
+int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, void* d_stats, void* d_ws, hipStream_t st) {
+  ChoiceArgs a{};
+  const ChoicePlan p = choice_plan(sc.rows, sc.M, dtype);
+  a.sc = sc;
+  a.splits = p.splits;
+  a.stats = d_stats;
+  a.ws = d_ws;
+  choice_launch(dtype, a, p, st);
+  GPX_HIP(ctx, hipGetLastError());
+  return 0;
+}
+
+} // namespace gpx
+
+extern "C" {
+
+int64_t gpx_choice_workspace(int64_t pools, int64_t rows, int64_t candidates, int dtype, int top) {
+  if (pools < 0 || rows < 0 || candidates < 0 || top < 0 || top > TOP_MAX || dtype < GPX_DTYPE_F64 || dtype > GPX_DTYPE_F16) return -1;
+  return choice_workspace(pools * rows, candidates, dtype, top);
+}
+
+int gpx_choice_logprobs(gpx_ctx* ctx, const gpx_scores* scores, const int64_t* d_choices, int64_t nchoices, int top,
+                        void* d_logprobs, void* d_entropy, void* d_logsumexp, void* d_stats, int64_t* d_top_indices,
+                        void* d_top_logprobs, void* d_workspace, int64_t workspace_bytes, void* stream) {
+  if (!ctx || ctx->device < 0) return -1;
+  ChoiceArgs a{};
+  GPX_TRY(pool_scores_view(ctx, scores, &a.sc, "gpx_choice_logprobs"));
+  if (nchoices < 0 || nchoices > INT32_MAX - 1024) return bad_arg(ctx, "gpx_choice_logprobs: number of choices");
+  if (top < 0 || top > TOP_MAX) return bad_arg(ctx, "gpx_choice_logprobs: top must be 0..64");
+  if (a.sc.rows == 0) return 0;
+  if (nchoices > 0 && (!d_choices || !d_logprobs)) return bad_arg(ctx, "gpx_choice_logprobs: null choices");
+  if (top > 0 && (!d_top_indices || !d_top_logprobs)) return bad_arg(ctx, "gpx_choice_logprobs: null alternatives");
+  if (!d_entropy || !d_logsumexp || !d_stats) return bad_arg(ctx, "gpx_choice_logprobs: null output");
+  const ChoicePlan p = choice_plan(a.sc.rows, a.sc.M, scores->dtype);
+  const int64_t need = choice_workspace(a.sc.rows, a.sc.M, scores->dtype, top);
+  if (need > 0 && (!d_workspace || workspace_bytes < need)) return bad_arg(ctx, "gpx_choice_logprobs: workspace too small (gpx_choice_workspace)");
+  a.choices = d_choices;
+  a.C = (int)nchoices;
+  a.top = top;
+  a.splits = p.splits;
+  a.logprobs = d_logprobs;
+  a.entropy = d_entropy;
+  a.lse = d_logsumexp;
+  a.stats = d_stats;
+  a.top_indices = d_top_indices;
+  a.top_logprobs = d_top_logprobs;
+  a.ws = d_workspace;
+  DeviceGuard g(ctx->device);
+  GPX_HIP(ctx, g.err);
+  choice_launch(scores->dtype, a, p, static_cast<hipStream_t>(stream));
+  GPX_HIP(ctx, hipGetLastError());
+  return 0;
+}
+
+int gpx_choice_logprobs_grad(gpx_ctx* ctx, const gpx_scores* scores, const int64_t* d_choices, int64_t nchoices,
+                             const void* d_logprobs, const void* d_grad_logprobs, int top, const int64_t* d_top_indices,
+                             const void* d_grad_top, const void* d_entropy, const void* d_stats, const void* d_grad_entropy,
+                             const void* d_grad_logsumexp, void* d_grad_scores, void* stream) {
+  if (!ctx || ctx->device < 0) return -1;
+  GradArgs a{};
+  GPX_TRY(pool_scores_view(ctx, scores, &a.sc, "gpx_choice_logprobs_grad"));
+  if (nchoices < 0 || nchoices > INT32_MAX - 1024) return bad_arg(ctx, "gpx_choice_logprobs_grad: number of choices");
+  if (top < 0 || top > TOP_MAX) return bad_arg(ctx, "gpx_choice_logprobs_grad: top must be 0..64");
+  if (a.sc.rows == 0 || a.sc.M == 0) return 0;
+  if (!d_stats || !d_grad_scores) return bad_arg(ctx, "gpx_choice_logprobs_grad: null statistics or gradient");
+  if (d_grad_logprobs && nchoices > 0 && (!d_choices || !d_logprobs)) return bad_arg(ctx, "gpx_choice_logprobs_grad: null choices");
+  if (d_grad_top && top > 0 && !d_top_indices) return bad_arg(ctx, "gpx_choice_logprobs_grad: null alternatives");
+  if (d_grad_entropy && !d_entropy) return bad_arg(ctx, "gpx_choice_logprobs_grad: null entropy");
+  a.choices = d_choices;
+  a.C = (int)nchoices;
+  a.logprobs = d_logprobs;
+  a.g_logprobs = nchoices > 0 ? d_grad_logprobs : nullptr;
+  a.top_indices = d_top_indices;
+  a.top = top;
+  a.g_top = top > 0 ? d_grad_top : nullptr;
+  a.entropy = d_entropy;
+  a.stats = d_stats;
+  a.g_entropy = d_grad_entropy;
+  a.g_lse = d_grad_logsumexp;
+  a.grad = d_grad_scores;
+  const int per = 64 * (scores->dtype == GPX_DTYPE_F64 || scores->dtype == GPX_DTYPE_F32 ? 8 : 16);
+  a.stretches = (a.sc.M + per - 1) / per;
+  const int64_t units = a.sc.rows * a.stretches;
+  const int64_t groups = (units + 3) / 4, gx = groups < (1 << 22) ? groups : (1 << 22), gy = (groups + gx - 1) / gx;
+  if (gy > 65535) return bad_arg(ctx, "gpx_choice_logprobs_grad: too many scores");
+  DeviceGuard g(ctx->device);
+  GPX_HIP(ctx, g.err);
+  const dim3 grid((unsigned)gx, (unsigned)gy), block(256);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (scores->dtype) {
+    case GPX_DTYPE_F64: hipLaunchKernelGGL(choice_grad_kernel<double>, grid, block, 0, st, a); break;
+    case GPX_DTYPE_F32: hipLaunchKernelGGL(choice_grad_kernel<float>, grid, block, 0, st, a); break;
+    case GPX_DTYPE_BF16: hipLaunchKernelGGL(choice_grad_kernel<bf16_t>, grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL(choice_grad_kernel<f16_t>, grid, block, 0, st, a); break;
+  }
+  GPX_HIP(ctx, hipGetLastError());
+  return 0;
+}
+
+} // extern "C"

@@ -295,6 +295,7 @@ struct gpx_ctx {
 
   // ---- generic scratch for unit-test entry points ---------------------------------------
   gpx::DevBuf tA, tB, tC;
+  gpx::DevBuf pool_scratch; // gpx_scratch: staging of host arrays for the pool operators
 
   // ---- profiling ------------------------------------------------------------------------
   bool prof_on = false;

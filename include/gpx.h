@@ -378,6 +378,83 @@ int gpx_gemm_nt(gpx_ctx* ctx, int M, int N, int K, double alpha, const double* A
  * out: L (n x n lower, zeros above).  *info as above. */
 int gpx_potrf(gpx_ctx* ctx, int n, const double* A, double* L, int* info);
 
+/* ---- operators over a pool of candidates: what follows the predictive sweep in a Bayesian-optimisation step ----------
+ * (the consumers of predict, gpax/acquisition/acquisition.py:22-35: the reference takes the argmax of the acquisition
+ * values, or of one draw, on the host; gpax/hypo.py:115-167 chooses by a softmax over the rewards).
+ * A row of scores (acquisition values, or one posterior draw) over a pool of candidates is a softmax policy
+ * p_j = exp(x_j / T) / sum_i exp(x_i / T).
+ *
+ * These entry points take DEVICE pointers and a stream of the context's device and return without waiting; they keep
+ * nothing in the context (workspaces are the caller's; one per call in flight), may be called while a stream is captured,
+ * and leave the caller's current device as it was.  The binding stages host arrays with gpx_scratch / gpx_upload /
+ * gpx_download on gpx_stream.
+ *
+ * Scores are pools x rows x candidates of any strides (in elements; 0 = broadcast), in float64, float32, bfloat16 or
+ * float16; statistics and other real arguments and results are float64 for float64 scores and float32 for the others ("the
+ * accumulator's type").  A candidate exists for a row if it lies below the row's length, its mask byte is nonzero and its
+ * score is not -inf; what is stored in the other places is never used.  A row in which nothing exists has log probabilities
+ * -inf, entropy 0, log-sum-exp -inf, no alternatives, gradient 0 and adds no weight.  A NaN or +inf score that exists, or a
+ * temperature on the device that is not positive and finite, makes its row NaN. */
+#define GPX_DTYPE_F64 0
+#define GPX_DTYPE_F32 1
+#define GPX_DTYPE_BF16 2
+#define GPX_DTYPE_F16 3
+typedef struct gpx_scores {
+  const void* d_scores;
+  int64_t pools, rows, candidates;
+  int64_t scores_stride[3];
+  const uint8_t* d_mask; /* or NULL */
+  int64_t mask_stride[3];
+  const void* d_lengths; /* per row, or NULL: the whole pool; clamped to [0, candidates] */
+  int64_t lengths_stride[2];
+  const void* d_temperatures; /* per row, of the accumulator's type, or NULL: `temperature` */
+  int64_t temperatures_stride[2];
+  double temperature;
+  int dtype;      /* GPX_DTYPE_* of the scores */
+  int lengths_64; /* lengths are int64 (else int32) */
+} gpx_scores;
+
+/* Bytes of workspace that gpx_choice_logprobs needs (0: none); host only.  < 0: bad arguments. */
+int64_t gpx_choice_workspace(int64_t pools, int64_t rows, int64_t candidates, int dtype, int top);
+/* Per row: log probabilities of `nchoices` given candidates (choices: rows x nchoices, contiguous; -1 = a filler, log
+ * probability 0; any other number outside the pool: NaN; a candidate that does not exist: -inf), the entropy, the log of
+ * the sum of exponentials of x / T, and the `top` <= 64 best candidates with their log probabilities (score descending,
+ * equal scores by index; index -1, log probability -inf where fewer exist; NaN scores are not among them).  d_stats
+ * (2 per row) is what gpx_choice_logprobs_grad reads. */
+int gpx_choice_logprobs(gpx_ctx* ctx, const gpx_scores* scores, const int64_t* d_choices, int64_t nchoices, int top,
+                        void* d_logprobs, void* d_entropy, void* d_logsumexp, void* d_stats, int64_t* d_top_indices,
+                        void* d_top_logprobs, void* d_workspace, int64_t workspace_bytes, void* stream);
+/* Gradient with respect to the scores (rows x candidates, contiguous, of the scores' type; rounded once) of
+ *   sum grad_logprobs * logprobs + grad_entropy * entropy + grad_logsumexp * logsumexp + sum grad_top * top_logprobs
+ * given the forward call's arguments and results; each of the four may be NULL.  The selection of alternatives is held
+ * fixed.  Fillers, and choices of log probability -inf, have no gradient; equal choices add up in their order. */
+int gpx_choice_logprobs_grad(gpx_ctx* ctx, const gpx_scores* scores, const int64_t* d_choices, int64_t nchoices,
+                             const void* d_logprobs, const void* d_grad_logprobs, int top, const int64_t* d_top_indices,
+                             const void* d_grad_top, const void* d_entropy, const void* d_stats, const void* d_grad_entropy,
+                             const void* d_grad_logsumexp, void* d_grad_scores, void* stream);
+/* Weight that each candidate of each pool has gathered: out = decay * weights + sum over the pool's rows of
+ * row_weight * p (pools x candidates, contiguous; weights NULL: zeros; row_weights pools x rows contiguous, NULL: ones; a row
+ * of weight 0 is not read).  out may be weights.  The sums have a fixed order.  Workspace as above. */
+int64_t gpx_pool_weights_workspace(int64_t pools, int64_t rows, int64_t candidates, int dtype);
+int gpx_pool_weights(gpx_ctx* ctx, const gpx_scores* scores, const void* d_row_weights, const void* d_weights, double decay,
+                     void* d_out, void* d_workspace, int64_t workspace_bytes, void* stream);
+/* Cuts every pool (its first lengths[b] candidates; lengths NULL: all) to at most `budget`: the `first` first and the
+ * `recent` last ones stay (first + recent <= budget), of the others those of largest weight (float64 or float32; equal
+ * weights: the lower index; NaN: the smallest).  What stays keeps its order: indices (pools x budget, -1 behind the last),
+ * new_lengths, weights, and the rows of up to 16 payload arrays (pools x candidates x payload_row_bytes, contiguous) are
+ * written to the outputs, with zeros behind the last.  The arrays of payload pointers are host arrays; outputs must not
+ * overlap inputs. */
+int gpx_pool_evict(gpx_ctx* ctx, int dtype, int64_t pools, int64_t candidates, const void* d_weights, const void* d_lengths,
+                   int lengths_64, int64_t lengths_stride, int64_t budget, int64_t first, int64_t recent, int64_t* d_indices,
+                   int64_t* d_new_lengths, void* d_weights_out, int npayload, const void* const* d_payload,
+                   void* const* d_payload_out, const int64_t* payload_row_bytes, void* stream);
+/* Staging of host arrays for the above: scratch of the context (valid until the next gpx_scratch, which waits for the
+ * context's stream), blocking copies, and that stream. */
+int gpx_scratch(gpx_ctx* ctx, int64_t bytes, void** d_out);
+int gpx_upload(gpx_ctx* ctx, void* d_dst, const void* src, int64_t bytes);
+int gpx_download(gpx_ctx* ctx, void* dst, const void* d_src, int64_t bytes);
+void* gpx_stream(gpx_ctx* ctx);
+
 #ifdef __cplusplus
 }
 #endif

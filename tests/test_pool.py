@@ -1,0 +1,171 @@
+"""CPU: argument handling, refusals and staging of the operators over a pool of candidates, with a stand-in engine on host
+memory (tests/pool_engine.py); the plain implementations themselves against differences; the compiled code."""
+import math
+import os
+import re
+import subprocess
+
+import numpy as np
+import pytest
+
+from gpax_amd import _lib
+from gpax_amd import acquisition as acq
+from tests import pool_oracle as ref
+from tests.pool_engine import PoolEngine
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(autouse=True)
+def engine():
+    _lib.set_engine(PoolEngine())
+    yield
+    _lib.set_engine(None)
+
+
+def test_the_plain_gradient_is_that_of_the_plain_results():
+    rng = np.random.default_rng(0)
+    x, mask, c, T = rng.standard_normal((3, 20)), rng.random((3, 20)) > 0.2, rng.integers(-1, 20, (3, 4)), 0.7
+    f = ref.choice(x, c, T, mask, None, 3)
+    gs = [rng.standard_normal(s) for s in ((3, 4), 3, 3, (3, 3))]
+    g, _ = ref.grad(x, f, c, *gs, T=T)
+
+    def F(x):
+        q = ref.choice(x, c, T, mask, None, 3)
+        return ((gs[0] * np.where(np.isfinite(q["logprobs"]), q["logprobs"], 0)).sum() + (gs[1] * q["entropy"]).sum()
+                + (gs[2] * q["logsumexp"]).sum() + (gs[3] * q["top_logprobs"]).sum())
+
+    h = 1e-5  # third derivatives below 30: h^2 / 6 x 30 = 5e-10; rounding 2^-53 x 200 x 30 / h = 7e-8
+    for i in range(3):
+        for j in range(20):
+            up, dn = x.copy(), x.copy()
+            up[i, j] += h
+            dn[i, j] -= h
+            assert abs((F(up) - F(dn)) / (2 * h) - g[i, j]) < 1e-7
+
+
+def test_plain_results_of_a_row_by_hand():
+    x = np.log(np.array([1.0, 2.0, 5.0, 8.0]))
+    f = ref.choice(x, np.array([2, -1, 3]), 1.0, np.array([1, 1, 1, 0]), None, 4)
+    p = np.array([1, 2, 5]) / 8
+    np.testing.assert_allclose(f["logprobs"][0], [np.log(p[2]), 0, -np.inf])
+    np.testing.assert_allclose(f["entropy"], -(p * np.log(p)).sum())
+    np.testing.assert_allclose(f["logsumexp"], np.log(8.0))
+    assert f["top_indices"][0].tolist() == [2, 1, 0, -1] and np.isneginf(f["top_logprobs"][0, 3])
+    assert ref.evict(np.array([0.1, 0.5, 0.5, 0.0, 0.2]), 3, (), 1, 1)[0].tolist() == [0, 1, 4]
+
+
+@pytest.mark.parametrize("shape", [(9,), (4, 9), (2, 3, 9), (0, 9), (3, 0)], ids=str)
+@pytest.mark.parametrize("kind", ["float64", "float32", "float16"])
+def test_staging_of_every_argument(shape, kind):
+    rng = np.random.default_rng(1)
+    lead, M = shape[:-1], shape[-1]
+    acc = "float64" if kind == "float64" else "float32"
+    x = rng.standard_normal(shape).astype(kind)
+    for mask in [None, rng.random(M) > 0.3, (rng.random(shape) > 0.3).astype(np.uint8)]:
+        for lengths in [None, np.asarray(rng.integers(0, M + 1, lead)), np.asarray(rng.integers(0, M + 1, lead[-1:] or ()), dtype=np.int32)]:
+            for T in [0.5, rng.uniform(0.5, 2, lead).astype(acc)]:
+                C = 2 if M else 0
+                c = rng.integers(-1, M, lead + (2,)) if M else None
+                r = acq.choice_logprobs(x, c, temperature=T, mask=mask, lengths=lengths, top=3)
+                f = ref.choice(x, c, T, mask, lengths, 3)
+                tol = dict(rtol=1e-6, atol=1e-6)
+                np.testing.assert_allclose(r.entropy.reshape(-1), f["entropy"], **tol)
+                np.testing.assert_array_equal(r.top_indices.reshape(-1, 3), f["top_indices"])
+                assert r.logprobs.shape == lead + (C,) and r.logprobs.dtype == acc and r.entropy.shape == lead
+                g = acq.choice_logprobs_grad(x, r, c, grad_logprobs=np.ones(lead + (C,), acc) if C else None, grad_entropy=np.ones(lead, acc),
+                                             temperature=T, mask=mask, lengths=lengths)
+                want, _ = ref.grad(x, f, c, np.ones(lead + (C,)) if C else None, np.ones(lead), T=T)
+                np.testing.assert_allclose(g.reshape(want.shape), want, rtol=2e-3, atol=2e-3 if kind == "float16" else 1e-6)
+                w = acq.pool_weights(x, temperature=T, mask=mask, lengths=lengths)
+                np.testing.assert_allclose(w, ref.weights(x, None, 1.0, None, T, mask, lengths), **tol)
+                assert w.shape == (shape[:1] + (M,) if len(shape) == 3 else (M,))
+
+
+def test_one_choice_a_row_and_lists():
+    r = acq.choice_logprobs([[0, 1], [2, 3]], [1, 0])
+    np.testing.assert_allclose(r.logprobs, [-math.log(1 + math.exp(-1)), -1 - math.log(1 + math.exp(-1))])
+    assert acq.choice_logprobs([0.0, 1.0], 1).logprobs.shape == ()
+
+
+def test_eviction_moves_points_and_reports_lengths():
+    w = np.array([[0.1, 0.9, 0.2, 0.8, 0.3], [1.0, 2.0, 3.0, 4.0, 5.0]])
+    pts = np.arange(20.0).reshape(2, 5, 2)
+    e = acq.pool_evict(w, 3, (pts,), recent=1, lengths=np.array([5, 2]))
+    assert e.indices.tolist() == [[1, 3, 4], [0, 1, -1]] and e.lengths.tolist() == [3, 2]
+    np.testing.assert_array_equal(e.payload[0][0], pts[0, [1, 3, 4]])
+    assert not e.payload[0][1, 2].any() and e.weights[1].tolist() == [1.0, 2.0, 0.0]
+    one = acq.pool_evict(w[0], 2, (pts[0].astype(np.float32), np.arange(5)))
+    assert one.indices.tolist() == [1, 3] and one.lengths.shape == () and one.payload[1].tolist() == [1, 3]
+
+
+X = np.zeros((3, 10))
+BAD = {
+    "four dimensions": lambda: acq.choice_logprobs(X[None, None]), "a scalar": lambda: acq.choice_logprobs(np.float64(1)),
+    "text": lambda: acq.choice_logprobs(np.array(["a"])), "complex": lambda: acq.choice_logprobs(X + 0j),
+    "top": lambda: acq.choice_logprobs(X, top=65), "negative top": lambda: acq.choice_logprobs(X, top=-1),
+    "temperature 0": lambda: acq.choice_logprobs(X, temperature=0), "temperature nan": lambda: acq.choice_logprobs(X, temperature=math.nan),
+    "temperature that 32 bits do not hold": lambda: acq.choice_logprobs(X.astype(np.float32), temperature=1e-50),
+    "temperature array": lambda: acq.choice_logprobs(X, temperature=np.array([1.0, -1.0, 1.0])),
+    "temperature shape": lambda: acq.choice_logprobs(X, temperature=np.ones(2)),
+    "mask shape": lambda: acq.choice_logprobs(X, mask=np.ones(9, bool)), "mask type": lambda: acq.choice_logprobs(X, mask=np.ones(10)),
+    "mask with more dimensions": lambda: acq.choice_logprobs(X, mask=np.ones((1, 3, 10), bool)),
+    "lengths shape": lambda: acq.choice_logprobs(X, lengths=np.ones(4, np.int64)), "lengths type": lambda: acq.choice_logprobs(X, lengths=np.ones(3)),
+    "choice beyond": lambda: acq.choice_logprobs(X, np.full((3, 1), 10)), "choice below": lambda: acq.choice_logprobs(X, np.full((3, 1), -2)),
+    "choice shape": lambda: acq.choice_logprobs(X, np.zeros((2, 1), int)), "choice type": lambda: acq.choice_logprobs(X, np.zeros((3, 1))),
+    "weights shape": lambda: acq.pool_weights(X, np.zeros(9)), "decay": lambda: acq.pool_weights(X, decay=-0.1),
+    "infinite decay": lambda: acq.pool_weights(X, decay=math.inf), "row weights": lambda: acq.pool_weights(X, row_weights=np.zeros(4)),
+    "out shape": lambda: acq.pool_weights(X, out=np.zeros(9)), "out type": lambda: acq.pool_weights(X, out=np.zeros(10, np.float32)),
+    "out strides": lambda: acq.pool_weights(X, out=np.zeros(20)[::2]),
+    "budget": lambda: acq.pool_evict(X, 0), "protected": lambda: acq.pool_evict(X, 4, first=3, recent=2), "negative": lambda: acq.pool_evict(X, 4, recent=-1),
+    "weights of three dimensions": lambda: acq.pool_evict(X[None], 4), "payload shape": lambda: acq.pool_evict(X, 4, (np.zeros((3, 9)),)),
+    "many payloads": lambda: acq.pool_evict(X, 4, (X,) * 17), "payload type": lambda: acq.pool_evict(X, 4, (np.full((3, 10), "a"),)),
+    "lengths of pools": lambda: acq.pool_evict(X, 4, lengths=np.ones(2, np.int64)),
+}
+
+
+@pytest.mark.parametrize("name", BAD)
+def test_refusals(name):
+    with pytest.raises(ValueError):
+        BAD[name]()
+
+
+def test_gradient_refusals():
+    r = acq.choice_logprobs(X, np.zeros((3, 1), int), top=2)
+    for kw in [dict(grad_logprobs=r.logprobs), dict(grad_entropy=np.zeros(4)), dict(grad_top_logprobs=np.zeros((3, 3)))]:
+        with pytest.raises(ValueError):
+            acq.choice_logprobs_grad(X, r, **kw)
+    with pytest.raises(ValueError):
+        acq.choice_logprobs_grad(X, tuple(r), grad_entropy=r.entropy)
+    with pytest.raises(ValueError):
+        acq.choice_logprobs_grad(X[:2], r, grad_entropy=r.entropy[:2])
+
+
+def test_tensors_on_the_host_are_refused():
+    torch = pytest.importorskip("torch")
+    with pytest.raises(ValueError):
+        acq.choice_logprobs(torch.zeros(3))
+    with pytest.raises(ValueError):
+        acq.choice_logprobs(X, mask=torch.ones(10, dtype=torch.bool))
+
+
+def test_workspace_sizes_come_from_sizes_alone():
+    lib = _lib.load_library()
+    assert lib.gpx_choice_workspace(1, 1000, 1024, 0, 8) == 0  # a row a wave
+    assert lib.gpx_choice_workspace(1, 1, 1 << 20, 0, 64) > 0  # several workgroups a row
+    assert lib.gpx_choice_workspace(1, -1, 4, 0, 0) < 0 and lib.gpx_choice_workspace(1, 1, 4, 9, 0) < 0 and lib.gpx_choice_workspace(1, 1, 4, 0, 65) < 0
+    assert lib.gpx_pool_weights_workspace(1, 1, 10, 0) == 0 and lib.gpx_pool_weights_workspace(1, 1000, 1024, 0) > 0
+    assert lib.gpx_pool_weights_workspace(-1, 1, 1, 0) < 0
+
+
+@pytest.mark.parametrize("source", ["choice.hip", "pool.hip"])
+def test_no_scalar_move_has_a_literal_of_more_than_32_bits(source, tmp_path):
+    """s_mov_b64 holds a literal of 32 bits; hipcc has emitted it with 64 (the double -inf), which loads 0."""
+    out = tmp_path / "k.s"
+    subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature",
+                    "-Xclang", "-packed-fp32-ops", "--cuda-device-only", "-S", os.path.join(ROOT, "gpax_amd", "csrc", source), "-o", str(out)],
+                   check=True, stderr=subprocess.DEVNULL)
+    text = out.read_text()
+    assert "s_endpgm" in text
+    bad = [m for m in re.findall(r"[sv]_mov_b64(?:_e32)? [sv]\[[0-9:]+\], (-?(?:0x[0-9a-f]+|[0-9]+))", text) if not -2 ** 31 <= int(m, 0) < 2 ** 32]
+    assert not bad, bad
