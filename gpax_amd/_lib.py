@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 from typing import Optional, Tuple
 
@@ -34,12 +35,8 @@ class GpxError(RuntimeError):
     pass
 
 
-class PoolScores(C.Structure):
-    """gpx_scores (include/gpx.h)."""
-    _fields_ = [("d_scores", C.c_void_p), ("pools", C.c_int64), ("rows", C.c_int64), ("candidates", C.c_int64),
-                ("scores_stride", C.c_int64 * 3), ("d_mask", C.c_void_p), ("mask_stride", C.c_int64 * 3),
-                ("d_lengths", C.c_void_p), ("lengths_stride", C.c_int64 * 2), ("d_temperatures", C.c_void_p),
-                ("temperatures_stride", C.c_int64 * 2), ("temperature", C.c_double), ("dtype", C.c_int), ("lengths_64", C.c_int)]
+# gpx_scores (include/gpx.h), packed by hand: a ctypes structure of 24 fields costs as much as the launch it describes
+POOL_SCORES = struct.Struct("@P3q3qP3qP2qP2qdii")
 
 
 def lib_path() -> str:
@@ -57,7 +54,7 @@ def load_library() -> C.CDLL:
             "(or `make -C gpax_amd/csrc`). gpax_amd has no CPU fallback."
         )
     lib = C.CDLL(_LIB_PATH)
-    vp, i64, scp = C.c_void_p, C.c_int64, C.POINTER(PoolScores)
+    vp, i64, scp = C.c_void_p, C.c_int64, C.c_char_p
     sig = {
         "gpx_init": (C.c_int, [C.c_int, C.POINTER(vp)]),
         "gpx_device_count": (C.c_int, []),
@@ -492,23 +489,23 @@ class Engine:
 
     # -- operators over a pool of candidates (gpax_amd/acquisition/pool.py prepares their arguments) ----------------
     # Addresses are device addresses (ints, 0 = none) on this engine's GPU; `stream` is a stream of it.  Nothing waits.
-    def choice_logprobs(self, scores: PoolScores, choices: int, nchoices: int, top: int, logprobs: int, entropy: int,
+    def choice_logprobs(self, scores: bytes, choices: int, nchoices: int, top: int, logprobs: int, entropy: int,
                         logsumexp: int, stats: int, top_indices: int, top_logprobs: int, workspace: int,
                         workspace_bytes: int, stream: int) -> None:
-        self._check(self._lib.gpx_choice_logprobs(self._ctx, C.byref(scores), choices, nchoices, top, logprobs, entropy,
+        self._check(self._lib.gpx_choice_logprobs(self._ctx, scores, choices, nchoices, top, logprobs, entropy,
                                                   logsumexp, stats, top_indices, top_logprobs, workspace, workspace_bytes,
                                                   stream), "gpx_choice_logprobs")
 
-    def choice_logprobs_grad(self, scores: PoolScores, choices: int, nchoices: int, logprobs: int, grad_logprobs: int,
+    def choice_logprobs_grad(self, scores: bytes, choices: int, nchoices: int, logprobs: int, grad_logprobs: int,
                              top: int, top_indices: int, grad_top: int, entropy: int, stats: int, grad_entropy: int,
                              grad_logsumexp: int, grad_scores: int, stream: int) -> None:
-        self._check(self._lib.gpx_choice_logprobs_grad(self._ctx, C.byref(scores), choices, nchoices, logprobs, grad_logprobs,
+        self._check(self._lib.gpx_choice_logprobs_grad(self._ctx, scores, choices, nchoices, logprobs, grad_logprobs,
                                                        top, top_indices, grad_top, entropy, stats, grad_entropy,
                                                        grad_logsumexp, grad_scores, stream), "gpx_choice_logprobs_grad")
 
-    def pool_weights(self, scores: PoolScores, row_weights: int, weights: int, decay: float, out: int, workspace: int,
+    def pool_weights(self, scores: bytes, row_weights: int, weights: int, decay: float, out: int, workspace: int,
                      workspace_bytes: int, stream: int) -> None:
-        self._check(self._lib.gpx_pool_weights(self._ctx, C.byref(scores), row_weights, weights, decay, out, workspace,
+        self._check(self._lib.gpx_pool_weights(self._ctx, scores, row_weights, weights, decay, out, workspace,
                                                workspace_bytes, stream), "gpx_pool_weights")
 
     def pool_evict(self, dtype: int, pools: int, candidates: int, weights: int, lengths: int, lengths_64: bool,

@@ -27,6 +27,11 @@ from .. import _lib
 MAX_TOP = 64
 MAX_PAYLOAD = 16
 _DTYPES = {"float64": 0, "float32": 1, "bfloat16": 2, "float16": 3}
+_INTS = ("int64", "int32")
+_MASKS = ("bool", "uint8")
+_pack = _lib.POOL_SCORES.pack
+_PAYLOAD = ("float64", "float32", "bfloat16", "float16", "float8_e4m3fn", "float8_e5m2", "int64", "int32", "int16", "int8",
+            "uint8", "bool", "complex64", "complex128")
 
 
 class ChoiceLogprobs(NamedTuple):
@@ -64,48 +69,68 @@ def _one_runtime() -> bool:
     return len(found) <= 1
 
 
+_torch = None  # torch, its types and the address of a stream, once a tensor has been seen (the package does not import it)
+_kind_of: dict = {}
+_type_of: dict = {}
+_stream_of = None
+
+
+def _bind_torch() -> None:
+    global _torch, _stream_of
+    torch = sys.modules["torch"]
+    if not _one_runtime():
+        raise _lib.GpxError("libgpx and torch have loaded two HIP runtimes: import torch before gpax_amd's library is loaded "
+                            "(before the first engine)")
+    for name in (*_DTYPES, *_INTS, *_MASKS, *_PAYLOAD):
+        _type_of[name] = getattr(torch, name)
+        _kind_of[_type_of[name]] = name
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # current_stream() without making a Stream object of it
+    _stream_of = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _torch = torch
+
+
 class _Device:
     """Torch tensors on one GPU."""
     host = False
 
     def __init__(self, ref):
-        self.torch = sys.modules["torch"]
-        if not isinstance(ref, self.torch.Tensor) or not ref.is_cuda:
+        if not getattr(ref, "is_cuda", False):
             raise ValueError("torch tensors must be on a GPU; pass NumPy arrays for data on the host")
-        if not _one_runtime():
-            raise _lib.GpxError("libgpx and torch have loaded two HIP runtimes: import torch before gpax_amd's library is "
-                                "loaded (before the first engine)")
-        self.ref, self.device = ref, ref.device
-        self.engine = _lib.get_device_engine(ref.device.index)
+        if _torch is None:
+            _bind_torch()
+        self.ref, self.index = ref, ref.get_device()
+        self.engine = _lib.get_device_engine(self.index)
 
     def take(self, a, name: str, kinds: Sequence[str], contiguous: bool = False):
-        if not isinstance(a, self.torch.Tensor) or a.device != self.device:
-            raise ValueError(f"{name} must be a torch tensor on {self.device}, as the first argument is")
-        kind = str(a.dtype)[6:]
-        if kind not in kinds:
-            raise ValueError(f"{name} has dtype {kind}; expected {' or '.join(kinds)}")
-        if a.requires_grad and self.torch.is_grad_enabled():
+        if not isinstance(a, _torch.Tensor) or a.get_device() != self.index:  # -1: on the host
+            raise ValueError(f"{name} must be a torch tensor on cuda:{self.index}, as the first argument is")
+        if _kind_of.get(a.dtype) not in kinds:
+            raise ValueError(f"{name} has dtype {a.dtype}; expected {' or '.join(kinds)}")
+        if a.requires_grad and _torch.is_grad_enabled():
             raise ValueError(f"{name} requires grad, and no graph is recorded: detach it and call choice_logprobs_grad")
-        if a.is_conj() or a.is_neg():
+        if a.is_neg():
             a = a.resolve_neg()
         return a.contiguous() if contiguous else a
 
     def kind(self, a) -> str:
-        return str(a.dtype)[6:]
+        return _kind_of[a.dtype]
 
     def strides(self, a):
         return a.stride()
 
     def new(self, shape, kind: str):
-        return self.ref.new_empty(shape, dtype=getattr(self.torch, kind), requires_grad=False)
+        return self.ref.new_empty(shape, dtype=_type_of[kind])
 
     def room(self, nbytes: int):
-        return self.new((nbytes,), "uint8") if nbytes else None
+        return self.ref.new_empty(nbytes, dtype=_type_of["uint8"]) if nbytes else None
 
     def run(self, inputs, outputs, fn, room=None) -> None:
-        stream = self.torch.cuda.current_stream(self.device).cuda_stream
         with self.engine._pool_lock:
-            fn(self.engine, lambda a: 0 if a is None else a.data_ptr(), stream)
+            fn(self.engine, _address, _stream_of(self.index))
+
+
+def _address(a) -> int:
+    return 0 if a is None else a.data_ptr()
 
 
 class _Room(NamedTuple):
@@ -166,6 +191,8 @@ def _space(a):
 
 def _broadcast_strides(shape, strides, to, name: str):
     """Strides that read an array of `shape` as one of shape `to`."""
+    if shape == to:
+        return strides
     lead = len(to) - len(shape)
     out = [0] * len(to)
     for i, (n, s) in enumerate(zip(shape, strides)):
@@ -175,8 +202,14 @@ def _broadcast_strides(shape, strides, to, name: str):
     return out
 
 
-def _padded(values, n: int):
-    return [0] * (n - len(values)) + list(values)
+def _pad3(v):
+    n = len(v)
+    return v if n == 3 else (0, v[0], v[1]) if n == 2 else (0, 0, v[0])
+
+
+def _pad2(v):
+    n = len(v)
+    return v if n == 2 else (0, v[0]) if n == 1 else (0, 0)
 
 
 class _Policy:
@@ -187,56 +220,54 @@ class _Policy:
         self.scores = x = space.take(scores, "scores", ("float64", "float32", "float16") if space.host else tuple(_DTYPES))
         if not 1 <= x.ndim <= 3:
             raise ValueError(f"scores have shape {tuple(x.shape)}; expected (M,), (rows, M) or (pools, rows, M)")
-        self.kind = space.kind(x)
-        self.acc = "float64" if self.kind == "float64" else "float32"
+        self.kind = kind = space.kind(x)
+        self.acc = acc = "float64" if kind == "float64" else "float32"
         self.shape = shape = tuple(x.shape)
-        self.lead, self.M = shape[:-1], shape[-1]
-        p, r = _padded(self.lead, 2) if len(shape) == 3 else (1, shape[0] if len(shape) == 2 else 1)
-        self.pools, self.rows = p, r
+        self.lead = lead = shape[:-1]
+        self.M = M = shape[-1]
+        self.pools, self.rows = p, r = lead if len(lead) == 2 else (1, lead[0]) if lead else (1, 1)
         if p * r > 1 << 25:
             raise ValueError("more than 2^25 rows of scores")
-        if self.M > (1 << 31) - 1 - 65536:
+        if M > (1 << 31) - 1 - 65536:
             raise ValueError("more than 2^31 - 65537 candidates")
         self.mask = self.lengths = self.temps = None
-        self.mask_strides = self.lengths_strides = self.temps_strides = ()
+        ms, ls, ts = (0, 0, 0), (0, 0), (0, 0)
+        n64 = 0
         if mask is not None:
-            self.mask = m = space.take(mask, "mask", ("bool", "uint8"))
-            self.mask_strides = _broadcast_strides(tuple(m.shape), space.strides(m), shape, "mask")
+            self.mask = m = space.take(mask, "mask", _MASKS)
+            ms = _pad3(_broadcast_strides(tuple(m.shape), space.strides(m), shape, "mask"))
         if lengths is not None:
-            self.lengths = n = space.take(lengths, "lengths", ("int64", "int32"))
-            self.lengths_strides = _broadcast_strides(tuple(n.shape), space.strides(n), self.lead, "lengths")
+            self.lengths = n = space.take(lengths, "lengths", _INTS)
+            ls = _pad2(_broadcast_strides(tuple(n.shape), space.strides(n), lead, "lengths"))
+            n64 = int(space.kind(n) == "int64")
         if isinstance(temperature, (int, float, np.number)):
-            self.temperature = float(temperature)
-            least = 2.3e-308 if self.acc == "float64" else 1.2e-38
-            if not (least <= self.temperature < math.inf) or (self.acc == "float32" and self.temperature > 3.4e38):
+            T = float(temperature)
+            if not (2.3e-308 <= T < math.inf if acc == "float64" else 1.2e-38 <= T <= 3.4e38):
                 raise ValueError("the temperature must be positive and finite")
         else:
-            self.temperature = 1.0
-            self.temps = t = space.take(temperature, "temperature", (self.acc,))
-            self.temps_strides = _broadcast_strides(tuple(t.shape), space.strides(t), self.lead, "temperature")
+            T = 1.0
+            self.temps = t = space.take(temperature, "temperature", (acc,))
+            ts = _pad2(_broadcast_strides(tuple(t.shape), space.strides(t), lead, "temperature"))
             if space.host and not (np.all(t > 0) and np.all(np.isfinite(t))):
                 raise ValueError("the temperature must be positive and finite")
+        self._rest = (p, r, M, *_pad3(space.strides(x))), ms, ls, (*ts, T, _DTYPES[kind], n64)
+
+    def struct(self, ptr) -> bytes:
+        a, ms, ls, rest = self._rest
+        return _pack(ptr(self.scores), *a, ptr(self.mask), *ms, ptr(self.lengths), *ls, ptr(self.temps), *rest)
 
     def inputs(self):
         return self.scores, self.mask, self.lengths, self.temps
 
-    def struct(self, ptr) -> "_lib.PoolScores":
-        return _lib.PoolScores(
-            ptr(self.scores), self.pools, self.rows, self.M, tuple(_padded(self.space.strides(self.scores), 3)),
-            ptr(self.mask) if self.mask is not None else 0, tuple(_padded(self.mask_strides, 3)),
-            ptr(self.lengths) if self.lengths is not None else 0, tuple(_padded(self.lengths_strides, 2)),
-            ptr(self.temps) if self.temps is not None else 0, tuple(_padded(self.temps_strides, 2)),
-            self.temperature, _DTYPES[self.kind], int(self.lengths is not None and self.space.kind(self.lengths) == "int64"))
-
     def choices(self, choices):
         """(choices, number per row, shape of the log probabilities)"""
         if choices is None:
-            return None, 0, self.lead + (0,)
+            return None, 0, None
         if isinstance(choices, (int, np.integer)) and self.space.host:
             choices = np.int64(choices)
-        c = self.space.take(choices, "choices", ("int64", "int32"), contiguous=True)
+        c = self.space.take(choices, "choices", _INTS, contiguous=True)
         shape = tuple(c.shape)
-        if shape != self.lead and shape[:-1] != self.lead or len(shape) > len(self.lead) + 1:
+        if shape != self.lead and (not shape or shape[:-1] != self.lead):
             raise ValueError(f"choices have shape {shape}; expected {self.lead} or {self.lead + ('C',)}")
         if self.space.kind(c) == "int32":
             c = c.astype(np.int64) if self.space.host else c.long()
@@ -270,8 +301,8 @@ def choice_logprobs(scores, choices=None, *, temperature=1.0, mask=None, lengths
         top: number of best alternatives to return, at most 64
 
     Returns:
-        ChoiceLogprobs: logprobs (as choices), entropy and logsumexp (one a row), top_indices and top_logprobs (rows, top):
-        score descending, equal scores by index, -1 and -inf where fewer exist; a row in which nothing exists has entropy 0
+        ChoiceLogprobs: logprobs (as choices; None without them), entropy and logsumexp (one a row), top_indices and
+        top_logprobs (rows, top; None for top = 0): score descending, equal scores by index, -1 and -inf where fewer exist; a row in which nothing exists has entropy 0
         and logsumexp -inf; a row with a NaN or +inf among what exists is NaN (NaN scores are never alternatives)
     """
     pol = _Policy(scores, temperature, mask, lengths)
@@ -280,9 +311,10 @@ def choice_logprobs(scores, choices=None, *, temperature=1.0, mask=None, lengths
         raise ValueError(f"top is {top}; expected 0 .. {MAX_TOP}")
     c, n, lp_shape = pol.choices(choices)
     sp = pol.space
-    logprobs, entropy, lse = sp.new(lp_shape, pol.acc), sp.new(pol.lead, pol.acc), sp.new(pol.lead, pol.acc)
-    stats = sp.new(pol.lead + (2,), pol.acc)
-    top_i, top_lp = sp.new(pol.lead + (top,), "int64"), sp.new(pol.lead + (top,), pol.acc)
+    lead, acc = pol.lead, pol.acc
+    logprobs = None if c is None else sp.new(lp_shape, acc)
+    entropy, lse, stats = sp.new(lead, acc), sp.new(lead, acc), sp.new(lead + (2,), acc)
+    top_i, top_lp = (sp.new(lead + (top,), "int64"), sp.new(lead + (top,), acc)) if top else (None, None)
     nbytes = _choice_workspace(pol.pools, pol.rows, pol.M, _DTYPES[pol.kind], top)
     ws = sp.room(nbytes)
 
@@ -336,6 +368,8 @@ def choice_logprobs_grad(scores, forward: ChoiceLogprobs, choices=None, *, grad_
     if grad_logsumexp is not None:
         g_lse = result(grad_logsumexp, "grad_logsumexp", pol.lead, (acc,))
     if grad_top_logprobs is not None:
+        if forward.top_indices is None:
+            raise ValueError("grad_top_logprobs needs the alternatives of the forward call")
         top = int(forward.top_indices.shape[-1])
         top_i = result(forward.top_indices, "forward.top_indices", pol.lead + (top,), ("int64",))
         g_top = result(grad_top_logprobs, "grad_top_logprobs", pol.lead + (top,), (acc,))
@@ -432,7 +466,7 @@ def pool_evict(weights, budget: int, payload: Sequence = (), *, first: int = 0, 
         raise ValueError("more than 2^19 - 1 pools, or 2^31 - 65537 candidates")
     n, n_stride, n64 = None, 0, False
     if lengths is not None:
-        n = sp.take(lengths, "lengths", ("int64", "int32"))
+        n = sp.take(lengths, "lengths", _INTS)
         stride = _broadcast_strides(tuple(n.shape), sp.strides(n), lead, "lengths")
         n_stride, n64 = (stride[0] if stride else 0), sp.kind(n) == "int64"
     payload = tuple(payload)
@@ -461,6 +495,3 @@ def pool_evict(weights, budget: int, payload: Sequence = (), *, first: int = 0, 
     sp.run((w, n, *moved), (indices, left, w_out, *moved_out), call)
     return PoolEviction(indices, left, w_out, tuple(moved_out))
 
-
-_PAYLOAD = ("float64", "float32", "bfloat16", "float16", "float8_e4m3fn", "float8_e5m2", "int64", "int32", "int16", "int8",
-            "uint8", "bool", "complex64", "complex128")

@@ -48,6 +48,33 @@ __device__ __forceinline__ bool before(A k1, uint32_t i1, A k2, uint32_t i2) {
   return k1 > k2 || (k1 == k2 && i1 < i2);
 }
 
+// Bitonic networks over the 64 lanes, best first, unrolled: the stage (SIZE, STRIDE) and all behind it.  From (2, 1) on it
+// sorts; from (64, 32) on it sorts what is a bitonic sequence already.
+template <int SIZE, int STRIDE, typename A>
+__device__ __forceinline__ void bitonic(A& k, uint32_t& i, int lane) {
+  const A ok = xor_lane<STRIDE>(k);
+  const uint32_t oi = xor_lane<STRIDE>(i);
+  const bool keep_first = ((lane & STRIDE) == 0) == ((lane & SIZE) == 0);
+  if (before(k, i, ok, oi) != keep_first) {
+    k = ok;
+    i = oi;
+  }
+  if constexpr (STRIDE > 1)
+    bitonic<SIZE, STRIDE / 2>(k, i, lane);
+  else if constexpr (SIZE < 64)
+    bitonic<SIZE * 2, SIZE>(k, i, lane);
+}
+template <int SIZE, int STRIDE, typename A>
+__device__ __forceinline__ void bitonic_values(A& v, int lane) {
+  const A o = xor_lane<STRIDE>(v);
+  const bool keep_first = ((lane & STRIDE) == 0) == ((lane & SIZE) == 0);
+  v = (v > o) == keep_first ? v : o;
+  if constexpr (STRIDE > 1)
+    bitonic_values<SIZE, STRIDE / 2>(v, lane);
+  else if constexpr (SIZE < 64)
+    bitonic_values<SIZE * 2, SIZE>(v, lane);
+}
+
 template <typename A>
 struct TopList {
   A key;        // lane l: the l-th best; -inf where there is none
@@ -65,20 +92,6 @@ struct TopList {
     thr_key = read_lane(key, k - 1);
     thr_idx = read_lane(idx, k - 1);
   }
-  static __device__ __forceinline__ void exchange(A& kk, uint32_t& ii, int stride, bool keep_first) {
-    const A ok = __shfl_xor(kk, stride);
-    const uint32_t oi = __shfl_xor(ii, stride);
-    if (before(kk, ii, ok, oi) != keep_first) {
-      kk = ok;
-      ii = oi;
-    }
-  }
-  static __device__ __forceinline__ void sort(A& kk, uint32_t& ii, int lane) {
-#pragma unroll 1
-    for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll 1
-      for (int stride = size >> 1; stride > 0; stride >>= 1) exchange(kk, ii, stride, ((lane & stride) == 0) == ((lane & size) == 0));
-  }
   // one sorted list into this one: the better of (mine, other reversed) lane by lane holds the best 64 of both as a bitonic
   // sequence, six exchanges sort it
   __device__ __forceinline__ void merge_sorted(A ck, uint32_t ci, int lane) {
@@ -88,10 +101,10 @@ struct TopList {
       key = rk;
       idx = ri;
     }
-#pragma unroll 1
-    for (int stride = 32; stride > 0; stride >>= 1) exchange(key, idx, stride, (lane & stride) == 0);
+    bitonic<64, 32>(key, idx, lane);
     rethreshold();
   }
+  // one candidate a lane (those that do not pass the threshold are dropped)
   __device__ __forceinline__ void consume(A x, uint32_t j, int lane) {
     const bool pass = x > neg_inf<A>() && before(x, j, thr_key, thr_idx); // NaN never passes
     uint64_t in = __ballot(pass);
@@ -99,7 +112,7 @@ struct TopList {
     if (__popcll(in) > INSERT_MAX) {
       A ck = pass ? x : neg_inf<A>();
       uint32_t ci = pass ? j : 0xffffffffu;
-      sort(ck, ci, lane);
+      bitonic<2, 1>(ck, ci, lane);
       merge_sorted(ck, ci, lane);
       return;
     }
@@ -125,6 +138,50 @@ struct TopList {
     merge_sorted(ck, ci, lane);
   }
 };
+
+// A step's candidates into the list.  Only those at or above a bound are looked at one by one: the list's threshold, or,
+// where at least k lanes hold something better, the k-th largest of the lanes' maxima (k candidates reach it, so no other can
+// be among the best k).  What passes is compacted in LDS (`slots`: the candidate's place in the step) and offered 64 at a time,
+// best estimate first come; the scores are read again, from the cache.
+template <typename T, int VEC, int U>
+__device__ __forceinline__ void offer_step(TopList<typename Acc<T>::type>& list, const typename Acc<T>::type* x, typename Acc<T>::type cm,
+                                           const Row<T>& v, int64_t j0, int lane, uint16_t* slots) {
+  typedef typename Acc<T>::type A;
+  // strictly above: a score equal to the k-th loses to it, whose index is lower (a wave takes its steps in order)
+  const uint64_t better = __ballot(cm > list.thr_key);
+  if (better == 0) return;
+  A bound = list.thr_key;
+  bool strict = true;
+  if (__popcll(better) >= list.k) {
+    A sorted = cm;
+    bitonic_values<2, 1>(sorted, lane);
+    bound = read_lane(sorted, list.k - 1);
+    strict = false;
+  }
+  int count = 0;
+#pragma unroll
+  for (int e = 0; e < U * VEC; ++e) {
+    const bool in = strict ? x[e] > bound : x[e] >= bound && x[e] > list.thr_key;
+    const uint64_t mask = __ballot(in);
+    if (mask) {
+      const int at = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+      if (in) slots[at] = (uint16_t)((e / VEC) * 64 * VEC + lane * VEC + e % VEC);
+      count += __popcll(mask);
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+  for (int i = 0; i < count; i += 64) {
+    A k = neg_inf<A>();
+    uint32_t j = 0xffffffffu;
+    if (i + lane < count) {
+      j = (uint32_t)(j0 + slots[i + lane]);
+      k = to_acc(v.x[j * v.xc]);
+    }
+    list.consume(k, j, lane);
+  }
+  __builtin_amdgcn_wave_barrier();
+}
 
 // What a row's statistics are turned into, by a team of `size` threads of which this one is `at`; the list by its wave.
 template <typename T>
@@ -187,11 +244,18 @@ __device__ __forceinline__ void join_waves(Stats<A>& st, TopList<A>& list, A c, 
   }
 }
 
-template <typename T, int WAVES, bool TOP>
+// Vectors that a lane has in flight: a step of 1024 candidates, or, for pools of at most 256 (512 of 16 bits), one of that
+// size: less code to fetch, which is most of what a launch of a few rows spends its time on.
+template <typename T>
+struct StepOf {
+  static constexpr int wide = 16 / VecOf<T>::value, narrow = sizeof(T) == 8 ? 2 : 1;
+};
+
+template <typename T, int WAVES, bool TOP, int U>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void choice_rows_kernel(ChoiceArgs a) {
   typedef typename Acc<T>::type A;
   constexpr int VEC = VecOf<T>::value;
-  constexpr int U = sizeof(T) == 8 ? 8 : 4;
+  __shared__ uint16_t sh_slots[TOP ? (WAVES == 1 ? 4 : WAVES) : 1][TOP ? U * VEC * 64 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
   if (row >= a.sc.rows) return; // WAVES == 1: whole waves, and no barrier below
@@ -211,15 +275,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void choice_rows_ker
 #pragma unroll
     for (int e = 1; e < U * VEC; ++e) cm = fmax(cm, x[e]);
     stats_add<A, U * VEC>(st, x, cm, c);
-    if (TOP) {
-      // strictly above: a score equal to the k-th loses to it, whose index is lower (steps are taken in order)
-      if (__ballot(cm > list.thr_key) != 0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) list.consume(x[u * VEC + e], (uint32_t)(j0 + u * 64 * VEC + lane * VEC + e), lane);
-      }
-    }
+    if constexpr (TOP) offer_step<T, VEC, U>(list, x, cm, v, j0, lane, sh_slots[wave]);
   }
   st = stats_wave(st, c);
   if constexpr (WAVES > 1) join_waves<A, WAVES, TOP>(st, list, c, wave, lane);
@@ -347,8 +403,7 @@ __global__ __launch_bounds__(256) void choice_grad_kernel(GradArgs a) {
   if (a.g_logprobs)
     gather(a.choices + row * a.C, static_cast<const A*>(a.g_logprobs) + row * a.C, static_cast<const A*>(a.logprobs) + row * a.C, a.C);
   if (a.g_top) gather(a.top_indices + row * a.top, static_cast<const A*>(a.g_top) + row * a.top, nullptr, a.top);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) G += __shfl_xor(G, o);
+  G = wave_sum(G);
   const A base = (a.g_lse ? static_cast<const A*>(a.g_lse)[row] : (A)0) - G;
   T* out = static_cast<T*>(a.grad) + row * a.sc.M;
 #pragma unroll
@@ -379,10 +434,9 @@ __global__ __launch_bounds__(256) void choice_grad_kernel(GradArgs a) {
 struct ChoicePlan {
   int waves, splits;
 };
-ChoicePlan choice_plan(int64_t rows, int64_t M, int dtype) {
+ChoicePlan choice_plan(int64_t rows, int64_t M) {
   constexpr int64_t TARGET = 4096;
-  const int64_t step = 64 * (dtype == GPX_DTYPE_F64 ? 16 : dtype == GPX_DTYPE_F32 ? 16 : 32);
-  const int64_t steps = (M + step - 1) / step;
+  const int64_t steps = (M + 1023) / 1024;
   int64_t want = rows > 0 ? (TARGET + rows - 1) / rows : 1;
   if (want > steps) want = steps;
   if (want <= 1) return ChoicePlan{1, 1};
@@ -396,12 +450,16 @@ ChoicePlan choice_plan(int64_t rows, int64_t M, int dtype) {
 template <typename T, bool TOP>
 void choice_launch(const ChoiceArgs& a, ChoicePlan p, hipStream_t st) {
   const unsigned rows = (unsigned)a.sc.rows;
+  constexpr int U = StepOf<T>::wide, UN = StepOf<T>::narrow;
   if (p.waves == 1) {
-    hipLaunchKernelGGL((choice_rows_kernel<T, 1, TOP>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
+    if (a.sc.M <= 64 * VecOf<T>::value * UN)
+      hipLaunchKernelGGL((choice_rows_kernel<T, 1, TOP, UN>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((choice_rows_kernel<T, 1, TOP, U>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
   } else if (p.waves == 16) {
-    hipLaunchKernelGGL((choice_rows_kernel<T, 16, TOP>), dim3(rows), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL((choice_rows_kernel<T, 16, TOP, U>), dim3(rows), dim3(1024), 0, st, a);
   } else {
-    hipLaunchKernelGGL((choice_rows_kernel<T, 4, TOP>), dim3(rows, p.splits), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((choice_rows_kernel<T, 4, TOP, U>), dim3(rows, p.splits), dim3(256), 0, st, a);
     if (p.splits > 1) hipLaunchKernelGGL((choice_join_kernel<T, 16, TOP>), dim3(rows), dim3(1024), 0, st, a);
   }
 }
@@ -422,7 +480,7 @@ void choice_launch(int dtype, const ChoiceArgs& a, ChoicePlan p, hipStream_t st)
 }
 int acc_size(int dtype) { return dtype == GPX_DTYPE_F64 ? 8 : 4; }
 int64_t choice_workspace(int64_t rows, int64_t M, int dtype, int top) {
-  const ChoicePlan p = choice_plan(rows, M, dtype);
+  const ChoicePlan p = choice_plan(rows, M);
   return p.splits == 1 ? 0 : rows * p.splits * partial_bytes(acc_size(dtype), top);
 }
 
@@ -464,7 +522,7 @@ int pool_scores_view(gpx_ctx* ctx, const gpx_scores* x, PoolScores* out, const c
 int64_t row_stats_workspace(int64_t rows, int64_t M, int dtype) { return choice_workspace(rows, M, dtype, 0); }
 int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, void* d_stats, void* d_ws, hipStream_t st) {
   ChoiceArgs a{};
-  const ChoicePlan p = choice_plan(sc.rows, sc.M, dtype);
+  const ChoicePlan p = choice_plan(sc.rows, sc.M);
   a.sc = sc;
   a.splits = p.splits;
   a.stats = d_stats;
@@ -495,7 +553,7 @@ int gpx_choice_logprobs(gpx_ctx* ctx, const gpx_scores* scores, const int64_t* d
   if (nchoices > 0 && (!d_choices || !d_logprobs)) return bad_arg(ctx, "gpx_choice_logprobs: null choices");
   if (top > 0 && (!d_top_indices || !d_top_logprobs)) return bad_arg(ctx, "gpx_choice_logprobs: null alternatives");
   if (!d_entropy || !d_logsumexp || !d_stats) return bad_arg(ctx, "gpx_choice_logprobs: null output");
-  const ChoicePlan p = choice_plan(a.sc.rows, a.sc.M, scores->dtype);
+  const ChoicePlan p = choice_plan(a.sc.rows, a.sc.M);
   const int64_t need = choice_workspace(a.sc.rows, a.sc.M, scores->dtype, top);
   if (need > 0 && (!d_workspace || workspace_bytes < need)) return bad_arg(ctx, "gpx_choice_logprobs: workspace too small (gpx_choice_workspace)");
   a.choices = d_choices;

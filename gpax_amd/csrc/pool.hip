@@ -68,8 +68,7 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
     A m = x[0];
 #pragma unroll
     for (int e = 1; e < PER_LANE; ++e) m = fmax(m, x[e]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o));
+    m = wave_max(m);
     if (WAVES > 1) { // two buffers: a row's values are overwritten two barriers after they were read
       if ((threadIdx.x & 63) == 0) red[flip][0][wave] = m;
       __syncthreads();
@@ -83,8 +82,7 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
       x[e] = exp2_acc((x[e] - ref) * c);
       s += x[e];
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    s = wave_sum(s);
     if (WAVES > 1) {
       if ((threadIdx.x & 63) == 0) red[flip][1][wave] = s;
       __syncthreads();

@@ -5,6 +5,7 @@ import threading
 
 import numpy as np
 
+from gpax_amd import _lib
 from tests import pool_oracle as ref
 from tests.oracle_engine import OracleEngine
 
@@ -42,12 +43,14 @@ class PoolEngine(OracleEngine):
         return 0
 
     def _read(self, s):
-        shape, kind = (s.pools, s.rows, s.candidates), KIND[s.dtype]
+        (d_scores, pools, rows, M, x0, x1, x2, d_mask, m0, m1, m2, d_lengths, l0, l1, d_temps, t0, t1, T, dtype,
+         n64) = _lib.POOL_SCORES.unpack(s)
+        shape, kind = (pools, rows, M), KIND[dtype]
         acc = "float64" if kind == "float64" else "float32"
-        x = view(s.d_scores, kind, shape, list(s.scores_stride))
-        mask = view(s.d_mask, "uint8", shape, list(s.mask_stride)) if s.d_mask else None
-        lengths = view(s.d_lengths, "int64" if s.lengths_64 else "int32", shape[:2], list(s.lengths_stride)) if s.d_lengths else None
-        T = view(s.d_temperatures, acc, shape[:2], list(s.temperatures_stride)) if s.d_temperatures else s.temperature
+        x = view(d_scores, kind, shape, [x0, x1, x2])
+        mask = view(d_mask, "uint8", shape, [m0, m1, m2]) if d_mask else None
+        lengths = view(d_lengths, "int64" if n64 else "int32", shape[:2], [l0, l1]) if d_lengths else None
+        T = view(d_temps, acc, shape[:2], [t0, t1]) if d_temps else T
         return x, mask, lengths, T, shape, acc
 
     def choice_logprobs(self, scores, choices, nchoices, top, logprobs, entropy, logsumexp, stats, top_indices, top_logprobs,
@@ -60,8 +63,9 @@ class PoolEngine(OracleEngine):
         view(logsumexp, acc, (n,))[...] = f["logsumexp"]
         if nchoices:
             view(logprobs, acc, (n, nchoices))[...] = f["logprobs"]
-        view(top_indices, "int64", (n, top))[...] = f["top_indices"]
-        view(top_logprobs, acc, (n, top))[...] = f["top_logprobs"]
+        if top:
+            view(top_indices, "int64", (n, top))[...] = f["top_indices"]
+            view(top_logprobs, acc, (n, top))[...] = f["top_logprobs"]
 
     def choice_logprobs_grad(self, scores, choices, nchoices, logprobs, grad_logprobs, top, top_indices, grad_top, entropy, stats,
                              grad_entropy, grad_logsumexp, grad_scores, stream):

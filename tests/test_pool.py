@@ -72,7 +72,8 @@ def test_staging_of_every_argument(shape, kind):
                 tol = dict(rtol=1e-6, atol=1e-6)
                 np.testing.assert_allclose(r.entropy.reshape(-1), f["entropy"], **tol)
                 np.testing.assert_array_equal(r.top_indices.reshape(-1, 3), f["top_indices"])
-                assert r.logprobs.shape == lead + (C,) and r.logprobs.dtype == acc and r.entropy.shape == lead
+                assert r.entropy.shape == lead and r.entropy.dtype == acc
+                assert r.logprobs is None if c is None else r.logprobs.shape == lead + (C,) and r.logprobs.dtype == acc
                 g = acq.choice_logprobs_grad(x, r, c, grad_logprobs=np.ones(lead + (C,), acc) if C else None, grad_entropy=np.ones(lead, acc),
                                              temperature=T, mask=mask, lengths=lengths)
                 want, _ = ref.grad(x, f, c, np.ones(lead + (C,)) if C else None, np.ones(lead), T=T)
