@@ -131,7 +131,8 @@ def load_library() -> C.CDLL:
         "gpx_pool_weights_workspace": (i64, [i64, i64, i64, C.c_int]),
         "gpx_pool_weights": (C.c_int, [vp, scp, vp, vp, C.c_double, vp, vp, i64, vp]),
         "gpx_pool_evict": (C.c_int, [vp, C.c_int, i64, i64, vp, vp, C.c_int, i64, i64, i64, i64, vp, vp, vp, C.c_int,
-                                     C.POINTER(vp), C.POINTER(vp), C.POINTER(i64), vp]),
+                                     C.POINTER(vp), C.POINTER(vp), C.POINTER(i64), vp, i64, vp]),
+        "gpx_pool_evict_workspace": (i64, [i64, i64, C.c_int]),
         "gpx_scratch": (C.c_int, [vp, i64, C.POINTER(vp)]),
         "gpx_upload": (C.c_int, [vp, vp, vp, i64]),
         "gpx_download": (C.c_int, [vp, vp, vp, i64]),
@@ -153,7 +154,7 @@ EXPORTED_SYMBOLS = (
     "gpx_potrf gpx_node_init gpx_node_destroy gpx_node_last_error gpx_node_info gpx_node_last_shares gpx_predict_sweep_multi "
     "gpx_rank_unique_id gpx_rank_init gpx_rank_destroy gpx_rank_last_error gpx_rank_info gpx_rank_device_pci gpx_rank_collective_calls gpx_rank_barrier gpx_rank_calibrate gpx_shard_ranges_weighted "
     "gpx_rank_allreduce_max gpx_rank_bcast gpx_rank_predict_sweep gpx_shard_range "
-    "gpx_choice_workspace gpx_choice_logprobs gpx_choice_logprobs_grad gpx_pool_weights_workspace gpx_pool_weights gpx_pool_evict "
+    "gpx_choice_workspace gpx_choice_logprobs gpx_choice_logprobs_grad gpx_pool_weights_workspace gpx_pool_weights gpx_pool_evict_workspace gpx_pool_evict "
     "gpx_scratch gpx_upload gpx_download gpx_stream"
 ).split()
 
@@ -510,12 +511,13 @@ class Engine:
 
     def pool_evict(self, dtype: int, pools: int, candidates: int, weights: int, lengths: int, lengths_64: bool,
                    lengths_stride: int, budget: int, first: int, recent: int, indices: int, new_lengths: int,
-                   weights_out: int, payload: list, payload_out: list, row_bytes: list, stream: int) -> None:
+                   weights_out: int, payload: list, payload_out: list, row_bytes: list, workspace: int,
+                   workspace_bytes: int, stream: int) -> None:
         n = len(payload)
         self._check(self._lib.gpx_pool_evict(self._ctx, dtype, pools, candidates, weights, lengths, int(lengths_64),
                                              lengths_stride, budget, first, recent, indices, new_lengths, weights_out, n,
                                              (C.c_void_p * n)(*payload), (C.c_void_p * n)(*payload_out),
-                                             (C.c_int64 * n)(*row_bytes), stream), "gpx_pool_evict")
+                                             (C.c_int64 * n)(*row_bytes), workspace, workspace_bytes, stream), "gpx_pool_evict")
 
     def scratch(self, nbytes: int) -> int:
         out = C.c_void_p()

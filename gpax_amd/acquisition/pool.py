@@ -35,14 +35,14 @@ _PAYLOAD = ("float64", "float32", "bfloat16", "float16", "float8_e4m3fn", "float
 
 
 class ChoiceLogprobs(NamedTuple):
-    """Results of `choice_logprobs`; `stats` (the row's largest score and the log2 of its sum) is what
-    `choice_logprobs_grad` reads."""
+    """Results of `choice_logprobs`.  The real ones are views of one array, `state`, which also holds what
+    `choice_logprobs_grad` reads of the forward pass."""
     logprobs: object
     entropy: object
     logsumexp: object
     top_indices: object
     top_logprobs: object
-    stats: object
+    state: object
 
 
 class PoolEviction(NamedTuple):
@@ -121,6 +121,12 @@ class _Device:
     def new(self, shape, kind: str):
         return self.ref.new_empty(shape, dtype=_type_of[kind])
 
+    def view(self, base, shape, offset: int):
+        """Contiguous part of a 1-D array: one allocation for several results costs half of one for each."""
+        n = len(shape)
+        stride = (1,) if n == 1 else (shape[1], 1) if n == 2 else (shape[1] * shape[2], shape[2], 1) if n == 3 else ()
+        return base.as_strided(shape, stride, offset)
+
     def room(self, nbytes: int):
         return self.ref.new_empty(nbytes, dtype=_type_of["uint8"]) if nbytes else None
 
@@ -165,6 +171,9 @@ class _Host:
     def new(self, shape, kind: str):
         return np.empty(shape, dtype=kind)
 
+    def view(self, base, shape, offset: int):
+        return base[offset:offset + math.prod(shape)].reshape(shape)
+
     def room(self, nbytes: int):
         return _Room(nbytes) if nbytes else None
 
@@ -193,6 +202,8 @@ def _broadcast_strides(shape, strides, to, name: str):
     """Strides that read an array of `shape` as one of shape `to`."""
     if shape == to:
         return strides
+    if len(shape) == 1 and shape[0] == to[-1]:
+        return (0,) * (len(to) - 1) + strides
     lead = len(to) - len(shape)
     out = [0] * len(to)
     for i, (n, s) in enumerate(zip(shape, strides)):
@@ -287,6 +298,11 @@ def _weights_workspace(pools, rows, M, dtype) -> int:
     return _lib.load_library().gpx_pool_weights_workspace(pools, rows, M, dtype)
 
 
+@functools.lru_cache(maxsize=4096)
+def _evict_workspace(pools, M, dtype) -> int:
+    return _lib.load_library().gpx_pool_evict_workspace(pools, M, dtype)
+
+
 def choice_logprobs(scores, choices=None, *, temperature=1.0, mask=None, lengths=None, top: int = 0) -> ChoiceLogprobs:
     """Softmax policy p_j = exp(x_j / T) / sum_i exp(x_i / T) over every row of scores, in one pass over them.
 
@@ -311,19 +327,22 @@ def choice_logprobs(scores, choices=None, *, temperature=1.0, mask=None, lengths
         raise ValueError(f"top is {top}; expected 0 .. {MAX_TOP}")
     c, n, lp_shape = pol.choices(choices)
     sp = pol.space
-    lead, acc = pol.lead, pol.acc
-    logprobs = None if c is None else sp.new(lp_shape, acc)
-    entropy, lse, stats = sp.new(lead, acc), sp.new(lead, acc), sp.new(lead + (2,), acc)
-    top_i, top_lp = (sp.new(lead + (top,), "int64"), sp.new(lead + (top,), acc)) if top else (None, None)
+    lead, rows = pol.lead, pol.pools * pol.rows
+    e, l, t, p = 2 * rows, 3 * rows, 4 * rows, (4 + top) * rows  # where the parts of `state` start; the statistics first
+    state = sp.new((p + n * rows,), pol.acc)
+    top_i = sp.new(lead + (top,), "int64") if top else None
     nbytes = _choice_workspace(pol.pools, pol.rows, pol.M, _DTYPES[pol.kind], top)
     ws = sp.room(nbytes)
+    size = 8 if pol.acc == "float64" else 4
 
     def call(engine, ptr, stream):
-        engine.choice_logprobs(pol.struct(ptr), ptr(c), n, top, ptr(logprobs), ptr(entropy), ptr(lse), ptr(stats), ptr(top_i),
-                               ptr(top_lp), ptr(ws), nbytes, stream)
+        base = ptr(state)
+        engine.choice_logprobs(pol.struct(ptr), ptr(c), n, top, base + p * size, base + e * size, base + l * size, base,
+                               ptr(top_i), base + t * size, ptr(ws), nbytes, stream)
 
-    sp.run((*pol.inputs(), c), (logprobs, entropy, lse, stats, top_i, top_lp), call, ws)
-    return ChoiceLogprobs(logprobs, entropy, lse, top_i, top_lp, stats)
+    sp.run((*pol.inputs(), c), (state, top_i), call, ws)
+    return ChoiceLogprobs(None if c is None else sp.view(state, lp_shape, p), sp.view(state, lead, e), sp.view(state, lead, l), top_i,
+                          sp.view(state, lead + (top,), t) if top else None, state)
 
 
 def choice_logprobs_grad(scores, forward: ChoiceLogprobs, choices=None, *, grad_logprobs=None, grad_entropy=None,
@@ -353,7 +372,9 @@ def choice_logprobs_grad(scores, forward: ChoiceLogprobs, choices=None, *, grad_
 
     if not isinstance(forward, ChoiceLogprobs):
         raise ValueError("forward must be what choice_logprobs returned")
-    stats = result(forward.stats, "forward.stats", pol.lead + (2,), (acc,))
+    state = sp.take(forward.state, "forward.state", (acc,), contiguous=True)
+    if state.ndim != 1 or state.shape[0] < 4 * pol.pools * pol.rows:
+        raise ValueError("forward is not the forward call on these scores")
     logprobs = entropy = top_i = None
     g_lp = g_h = g_lse = g_top = None
     top = 0
@@ -377,9 +398,9 @@ def choice_logprobs_grad(scores, forward: ChoiceLogprobs, choices=None, *, grad_
 
     def call(engine, ptr, stream):
         engine.choice_logprobs_grad(pol.struct(ptr), ptr(c), n, ptr(logprobs), ptr(g_lp), top, ptr(top_i), ptr(g_top),
-                                    ptr(entropy), ptr(stats), ptr(g_h), ptr(g_lse), ptr(grad), stream)
+                                    ptr(entropy), ptr(state), ptr(g_h), ptr(g_lse), ptr(grad), stream)
 
-    sp.run((*pol.inputs(), c, logprobs, g_lp, top_i, g_top, entropy, stats, g_h, g_lse), (grad,), call)
+    sp.run((*pol.inputs(), c, logprobs, g_lp, top_i, g_top, entropy, state, g_h, g_lse), (grad,), call)
     return grad
 
 
@@ -462,8 +483,8 @@ def pool_evict(weights, budget: int, payload: Sequence = (), *, first: int = 0, 
         raise ValueError(f"the budget is {budget}; expected a positive number")
     if first < 0 or recent < 0 or first + recent > budget:
         raise ValueError(f"first = {first} and recent = {recent} must not be negative, and together at most the budget {budget}")
-    if pools > (1 << 19) - 1 or M > (1 << 31) - 1 - 65536:
-        raise ValueError("more than 2^19 - 1 pools, or 2^31 - 65537 candidates")
+    if pools > 65535 or M > (1 << 31) - 1 - 65536:
+        raise ValueError("more than 65535 pools, or 2^31 - 65537 candidates")
     n, n_stride, n64 = None, 0, False
     if lengths is not None:
         n = sp.take(lengths, "lengths", _INTS)
@@ -488,10 +509,14 @@ def pool_evict(weights, budget: int, payload: Sequence = (), *, first: int = 0, 
             raise ValueError(f"payload[{i}] has rows of 2 GiB or more")
     indices, left, w_out = sp.new(lead + (budget,), "int64"), sp.new(lead, "int64"), sp.new(lead + (budget,), sp.kind(w))
 
-    def call(engine, ptr, stream):
-        engine.pool_evict(_DTYPES[sp.kind(w)], pools, M, ptr(w), ptr(n), n64, n_stride, budget, first, recent, ptr(indices),
-                          ptr(left), ptr(w_out), [ptr(a) for a in moved], [ptr(a) for a in moved_out], row_bytes, stream)
+    dtype = _DTYPES[sp.kind(w)]
+    nbytes = _evict_workspace(pools, M, dtype)
+    ws = sp.room(nbytes)
 
-    sp.run((w, n, *moved), (indices, left, w_out, *moved_out), call)
+    def call(engine, ptr, stream):
+        engine.pool_evict(dtype, pools, M, ptr(w), ptr(n), n64, n_stride, budget, first, recent, ptr(indices),
+                          ptr(left), ptr(w_out), [ptr(a) for a in moved], [ptr(a) for a in moved_out], row_bytes, ptr(ws), nbytes, stream)
+
+    sp.run((w, n, *moved), (indices, left, w_out, *moved_out), call, ws)
     return PoolEviction(indices, left, w_out, tuple(moved_out))
 

@@ -139,49 +139,58 @@ struct TopList {
   }
 };
 
-// A step's candidates into the list.  Only those at or above a bound are looked at one by one: the list's threshold, or,
-// where at least k lanes hold something better, the k-th largest of the lanes' maxima (k candidates reach it, so no other can
-// be among the best k).  What passes is compacted in LDS (`slots`: the candidate's place in the step) and offered 64 at a time,
-// best estimate first come; the scores are read again, from the cache.
+// The candidates of a step that may belong into the list.  Only those at or above a bound are looked at one by one: the list's
+// threshold, or, where at least k lanes hold something better, the k-th largest of the lanes' maxima (k candidates reach it, so
+// no other can be among the best k).  What passes is kept in LDS by its index and waits there until 64 are together, or the
+// row ends; then the scores are read again, from the cache, and offered 64 at a time.  A threshold that is not up to date only
+// lets more pass.
 template <typename T, int VEC, int U>
-__device__ __forceinline__ void offer_step(TopList<typename Acc<T>::type>& list, const typename Acc<T>::type* x, typename Acc<T>::type cm,
-                                           const Row<T>& v, int64_t j0, int lane, uint16_t* slots) {
+struct Waiting {
   typedef typename Acc<T>::type A;
-  // strictly above: a score equal to the k-th loses to it, whose index is lower (a wave takes its steps in order)
-  const uint64_t better = __ballot(cm > list.thr_key);
-  if (better == 0) return;
-  A bound = list.thr_key;
-  bool strict = true;
-  if (__popcll(better) >= list.k) {
-    A sorted = cm;
-    bitonic_values<2, 1>(sorted, lane);
-    bound = read_lane(sorted, list.k - 1);
-    strict = false;
-  }
-  int count = 0;
-#pragma unroll
-  for (int e = 0; e < U * VEC; ++e) {
-    const bool in = strict ? x[e] > bound : x[e] >= bound && x[e] > list.thr_key;
-    const uint64_t mask = __ballot(in);
-    if (mask) {
-      const int at = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
-      if (in) slots[at] = (uint16_t)((e / VEC) * 64 * VEC + lane * VEC + e % VEC);
-      count += __popcll(mask);
-    }
-  }
-  __builtin_amdgcn_wave_barrier();
+  uint32_t* idx; // U * VEC * 64 + 64 of this wave
+  int count;
+
+  __device__ __forceinline__ void flush(TopList<A>& list, const Row<T>& v, int lane) {
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-  for (int i = 0; i < count; i += 64) {
-    A k = neg_inf<A>();
-    uint32_t j = 0xffffffffu;
-    if (i + lane < count) {
-      j = (uint32_t)(j0 + slots[i + lane]);
-      k = to_acc(v.x[j * v.xc]);
+    for (int i = 0; i < count; i += 64) {
+      A k = neg_inf<A>();
+      uint32_t j = 0xffffffffu;
+      if (i + lane < count) {
+        j = idx[i + lane];
+        k = to_acc(v.x[j * v.xc]);
+      }
+      list.consume(k, j, lane);
     }
-    list.consume(k, j, lane);
+    __builtin_amdgcn_wave_barrier();
+    count = 0;
   }
-  __builtin_amdgcn_wave_barrier();
-}
+  // a step; true: 64 or more wait
+  __device__ __forceinline__ bool step(const TopList<A>& list, const A* x, A cm, int64_t j0, int lane) {
+    // strictly above: a score equal to the k-th loses to it, whose index is lower (a wave takes its steps in order)
+    const uint64_t better = __ballot(cm > list.thr_key);
+    if (better == 0) return false;
+    A bound = list.thr_key;
+    bool strict = true;
+    if (__popcll(better) >= list.k) {
+      bound = cm;
+      bitonic_values<2, 1>(bound, lane);
+      bound = read_lane(bound, list.k - 1);
+      strict = false;
+    }
+#pragma unroll
+    for (int e = 0; e < U * VEC; ++e) {
+      const bool in = strict ? x[e] > bound : x[e] >= bound && x[e] > list.thr_key;
+      const uint64_t mask = __ballot(in);
+      if (mask) {
+        const int at = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+        if (in) idx[at] = (uint32_t)(j0 + (e / VEC) * 64 * VEC + lane * VEC + e % VEC);
+        count += __popcll(mask);
+      }
+    }
+    return count >= 64 || !strict; // with a bound of its own the step has much for the list: the threshold comes next
+  }
+};
 
 // What a row's statistics are turned into, by a team of `size` threads of which this one is `at`; the list by its wave.
 template <typename T>
@@ -255,7 +264,7 @@ template <typename T, int WAVES, bool TOP, int U>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void choice_rows_kernel(ChoiceArgs a) {
   typedef typename Acc<T>::type A;
   constexpr int VEC = VecOf<T>::value;
-  __shared__ uint16_t sh_slots[TOP ? (WAVES == 1 ? 4 : WAVES) : 1][TOP ? U * VEC * 64 : 1];
+  __shared__ uint32_t sh_waiting[TOP ? (WAVES == 1 ? 4 : WAVES) : 1][TOP ? U * VEC * 64 + 64 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
   if (row >= a.sc.rows) return; // WAVES == 1: whole waves, and no barrier below
@@ -265,6 +274,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void choice_rows_ker
   Stats<A> st = stats_empty<A>();
   TopList<A> list;
   if (TOP) list.init(a.top);
+  Waiting<T, VEC, U> waiting{sh_waiting[wave], 0};
   const int64_t step = (int64_t)64 * VEC * U;
   const int64_t first = WAVES == 1 ? 0 : ((int64_t)blockIdx.y * WAVES + wave) * step;
   const int64_t stride = WAVES == 1 ? step : (int64_t)a.splits * WAVES * step;
@@ -275,8 +285,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void choice_rows_ker
 #pragma unroll
     for (int e = 1; e < U * VEC; ++e) cm = fmax(cm, x[e]);
     stats_add<A, U * VEC>(st, x, cm, c);
-    if constexpr (TOP) offer_step<T, VEC, U>(list, x, cm, v, j0, lane, sh_slots[wave]);
+    if constexpr (TOP) {
+      if (waiting.step(list, x, cm, j0, lane)) waiting.flush(list, v, lane);
+    }
   }
+  if constexpr (TOP) waiting.flush(list, v, lane);
   st = stats_wave(st, c);
   if constexpr (WAVES > 1) join_waves<A, WAVES, TOP>(st, list, c, wave, lane);
   if (WAVES == 1 || a.splits == 1) {

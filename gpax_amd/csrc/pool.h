@@ -129,23 +129,26 @@ template <int S>
 __device__ __forceinline__ double xor_lane(double v) {
   return __hiloint2double((int)xor_lane<S>((uint32_t)__double2hiint(v)), (int)xor_lane<S>((uint32_t)__double2loint(v)));
 }
+template <int S>
+__device__ __forceinline__ uint64_t xor_lane(uint64_t v) {
+  return ((uint64_t)xor_lane<S>((uint32_t)(v >> 32)) << 32) | xor_lane<S>((uint32_t)v);
+}
+template <typename V, typename F>
+__device__ __forceinline__ V wave_reduce(V v, F f) {
+  v = f(v, xor_lane<32>(v));
+  v = f(v, xor_lane<16>(v));
+  v = f(v, xor_lane<8>(v));
+  v = f(v, xor_lane<4>(v));
+  v = f(v, xor_lane<2>(v));
+  return f(v, xor_lane<1>(v));
+}
 template <typename V>
 __device__ __forceinline__ V wave_max(V v) {
-  v = fmax(v, xor_lane<32>(v));
-  v = fmax(v, xor_lane<16>(v));
-  v = fmax(v, xor_lane<8>(v));
-  v = fmax(v, xor_lane<4>(v));
-  v = fmax(v, xor_lane<2>(v));
-  return fmax(v, xor_lane<1>(v));
+  return wave_reduce(v, [](V x, V y) { return fmax(x, y); });
 }
 template <typename V>
 __device__ __forceinline__ V wave_sum(V v) {
-  v += xor_lane<32>(v);
-  v += xor_lane<16>(v);
-  v += xor_lane<8>(v);
-  v += xor_lane<4>(v);
-  v += xor_lane<2>(v);
-  return v + xor_lane<1>(v);
+  return wave_reduce(v, [](V x, V y) { return x + y; });
 }
 
 template <typename A>

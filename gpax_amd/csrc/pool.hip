@@ -120,58 +120,78 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
 }
 
 // Second pass over longer pools: the rows' statistics are known, a workgroup sums 256 x VEC candidates over its share of rows.
+// The next four rows are on their way while four are worked on; a mask that all rows share is read once.
 template <typename T>
 __global__ __launch_bounds__(256) void pool_columns_kernel(WeightArgs a) {
   typedef typename Acc<T>::type A;
   constexpr int VEC = VecOf<T>::value, ROWS = 4;
-  const int64_t b = blockIdx.z;
-  const int64_t j0 = (int64_t)blockIdx.x * 256 * VEC;
+  const int64_t b = blockIdx.z, M = a.sc.M;
+  const int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
   const int64_t per = (a.sc.R + a.groups - 1) / a.groups;
-  const int64_t r1 = per * (blockIdx.y + 1) < a.sc.R ? per * (blockIdx.y + 1) : a.sc.R;
+  const int64_t r0 = per * blockIdx.y, r1 = r0 + per < a.sc.R ? r0 + per : a.sc.R;
   A acc[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = (A)0;
-  for (int64_t r = per * blockIdx.y; r < r1; r += ROWS) {
-    A x[ROWS][VEC];
-    Row<T> v[ROWS];
-    bool whole = true; // all of the rows' tile exists: their loads are in flight together
+  const bool whole = ((int64_t)blockIdx.x + 1) * 256 * VEC <= M && a.sc.xc == 1; // uniform: vectors, else score by score
+  const bool own_mask = a.sc.mask && a.sc.mr != 0;
+  const T* x = static_cast<const T*>(a.sc.x) + b * a.sc.xb;
+  const uint8_t* mask = a.sc.mask ? a.sc.mask + b * a.sc.mb : nullptr;
+  uint32_t shared = ~0u; // which of this lane's candidates the mask of all rows allows
+  if (mask && !own_mask)
 #pragma unroll
-    for (int q = 0; q < ROWS; ++q) { // past the last row: that row again, with weight 0
-      v[q] = row_view<T>(a.sc, b, r + q < r1 ? r + q : r1 - 1);
-      whole = whole && v[q].xc == 1 && (!v[q].mask || v[q].mc == 1) && j0 + 256 * VEC <= v[q].n;
-    }
-    if (whole) {
-      Pack<T, VEC> p[ROWS];
-      MaskPack<VEC> k[ROWS];
-#pragma unroll
-      for (int q = 0; q < ROWS; ++q) {
-        p[q] = *reinterpret_cast<const Pack<T, VEC>*>(v[q].x + j0 + threadIdx.x * VEC);
-        if (v[q].mask) k[q] = *reinterpret_cast<const MaskPack<VEC>*>(v[q].mask + j0 + threadIdx.x * VEC);
-      }
-#pragma unroll
-      for (int q = 0; q < ROWS; ++q)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) x[q][e] = !v[q].mask || k[q].v[e] ? to_acc(p[q].v[e]) : neg_inf<A>();
-    } else {
-#pragma unroll
-      for (int q = 0; q < ROWS; ++q) load_step<T, VEC, 1>(v[q], j0, 256 * VEC, threadIdx.x * VEC, x[q]);
-    }
+    for (int e = 0; e < VEC; ++e)
+      if (j + e >= M || !mask[(j + e) * a.sc.mc]) shared &= ~(1u << e);
+  auto load = [&](int64_t r, Pack<T, VEC>* p, uint32_t* ok) { // past the last row: the last one again, never used
 #pragma unroll
     for (int q = 0; q < ROWS; ++q) {
       const int64_t rq = r + q < r1 ? r + q : r1 - 1;
-      const int64_t row = b * a.sc.R + rq;
-      const A u = r + q >= r1 ? (A)0 : a.row_weights ? static_cast<const A*>(a.row_weights)[row] : (A)1;
+      const T* row = x + rq * a.sc.xr;
+      ok[q] = shared;
+      if (whole) {
+        p[q] = *reinterpret_cast<const Pack<T, VEC>*>(row + j);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) p[q].v[e] = row[(j + e < M ? j + e : M - 1) * a.sc.xc];
+      }
+      if (own_mask) {
+        const uint8_t* m = mask + rq * a.sc.mr;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (!m[(j + e < M ? j + e : M - 1) * a.sc.mc]) ok[q] &= ~(1u << e);
+      }
+    }
+  };
+  Pack<T, VEC> next[ROWS];
+  uint32_t next_ok[ROWS];
+  if (r0 < r1) load(r0, next, next_ok);
+  for (int64_t r = r0; r < r1; r += ROWS) {
+    Pack<T, VEC> p[ROWS];
+    uint32_t ok[ROWS];
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+      p[q] = next[q];
+      ok[q] = next_ok[q];
+    }
+    if (r + ROWS < r1) load(r + ROWS, next, next_ok);
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+      if (r + q >= r1) break; // uniform, as all of the row's quantities
+      const int64_t row = b * a.sc.R + r + q;
+      const A u = a.row_weights ? static_cast<const A*>(a.row_weights)[row] : (A)1;
       if (u == (A)0) continue;
-      const A c = temperature_scale(row_temperature<A>(a.sc, b, rq));
+      const A c = temperature_scale(row_temperature<A>(a.sc, b, r + q));
       const A m = static_cast<const A*>(a.stats)[2 * row], log2s = static_cast<const A*>(a.stats)[2 * row + 1];
+      const int n = row_length(a.sc, b, r + q);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const A p = u * exp2_acc((x[q][e] - m) * c - log2s);
-        acc[e] += x[q][e] == neg_inf<A>() ? (A)0 : p;
+        const A v = to_acc(p[q].v[e]);
+        const A w = u * exp2_acc((v - m) * c - log2s);
+        const bool in = j + e < n && ((ok[q] >> e) & 1) && v != neg_inf<A>();
+        acc[e] += in ? w : (A)0;
       }
     }
   }
-  store_sums<A, VEC>(a, b, blockIdx.y, j0 + threadIdx.x * VEC, acc);
+  store_sums<A, VEC>(a, b, blockIdx.y, j, acc);
 }
 
 // decay w + the groups' partial sums in their order: 64 candidates per workgroup, the groups dealt to its four waves
@@ -197,9 +217,25 @@ __global__ __launch_bounds__(256) void pool_weights_join_kernel(WeightArgs a) {
 }
 
 // ---- eviction ---------------------------------------------------------------------------------------------------------
+//
+// What stays of a pool of L > budget candidates: the `first` first, the `recent` last, and of the others the `need` of largest
+// weight.  The need-th largest is found on integers of the weights' order, digit by digit from the highest bit in which they
+// differ at all, by histograms; a digit that holds exactly what is still needed ends the search.  Candidates above the found
+// prefix stay, of those equal to it the first in order.  Counts only: no result depends on the order of an atomic.
+//
+// One workgroup per pool where the pool fits its registers (16384 candidates).  Longer pools are cut into chunks of 4096, a
+// workgroup each, over five launches: range of the keys | histogram of 12 bits | of the next 12 | the few candidates that
+// share all 24 (or that need no telling apart) | output.  Read five times, but 2 MB of weights stay in the caches: bound by
+// the launches.
 
-constexpr int EVICT_PER = 16, EVICT_CHUNK = 1024 * EVICT_PER;
+constexpr int EVICT_PAYLOADS = 16;
+constexpr int FUSED_ROW_BYTES = 64; // payload rows up to this are moved by the lane that keeps the candidate
 
+struct Payload {
+  const char* src;
+  char* dst;
+  int bytes, unit; // of a row; of one access
+};
 struct EvictArgs {
   const void* weights; // pools x M
   const void* lengths;
@@ -209,6 +245,10 @@ struct EvictArgs {
   int64_t* indices; // pools x K
   int64_t* new_lengths;
   void* out; // pools x K
+  int npay;
+  void* ws;
+  int64_t chunks;
+  Payload pay[EVICT_PAYLOADS];
 };
 
 // weights as integers of the same order; NaN lowest, -0 = +0
@@ -230,207 +270,604 @@ template <>
 struct KeyOf<double> {
   typedef uint64_t type;
 };
+// key >> shift where shift may be all of the key's bits
+template <typename Key>
+__device__ __forceinline__ Key above(Key k, int shift) {
+  return shift >= (int)sizeof(Key) * 8 ? (Key)0 : k >> (shift & (int)(sizeof(Key) * 8 - 1));
+}
+template <typename Key>
+__device__ __forceinline__ int bits_of(Key diff) {
+  return diff == 0 ? 0 : (int)sizeof(Key) * 8 - (sizeof(Key) == 8 ? __clzll((long long)diff) : __clz((int)diff));
+}
+
+template <typename V, typename F>
+__device__ __forceinline__ V block_reduce(V v, V* sh, F f) { // 16 waves; sh: 16 values, not reused before the next barrier
+  v = wave_reduce(v, f);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = sh[0];
+  for (int i = 1; i < 16; ++i) v = f(v, sh[i]);
+  return v;
+}
+template <typename Key>
+__device__ __forceinline__ Key key_and(Key x, Key y) {
+  return x & y;
+}
+template <typename Key>
+__device__ __forceinline__ Key key_or(Key x, Key y) {
+  return x | y;
+}
+
+struct PoolCut { // what a pool's length leaves to decide
+  int64_t L, keep, lo, hi; // candidates lo .. hi - 1 are free to go
+  uint32_t need;           // how many of them stay
+};
+__device__ __forceinline__ PoolCut pool_cut(const EvictArgs& a, int64_t b) {
+  PoolCut c;
+  c.L = a.M;
+  if (a.lengths) {
+    c.L = a.len64 ? static_cast<const int64_t*>(a.lengths)[b * a.ls] : (int64_t)static_cast<const int32_t*>(a.lengths)[b * a.ls];
+    c.L = c.L < 0 ? 0 : (c.L > a.M ? a.M : c.L);
+  }
+  const bool all = c.L <= a.K;
+  c.keep = all ? c.L : a.K;
+  c.lo = all ? 0 : a.first;
+  c.hi = all ? 0 : c.L - a.recent;
+  c.need = all ? 0u : (uint32_t)(a.K - a.first - a.recent);
+  return c;
+}
 
 struct Digit { // where the need-th largest lies in a histogram, counted from the top
   int bin;
   uint32_t above, count;
 };
-// 256 bins by one wave: lane l holds bins 4 l .. 4 l + 3
-__device__ __forceinline__ Digit find_digit(const uint32_t* hist, uint32_t need, int lane) {
+constexpr int WIDE_BITS = 12, WIDE_BINS = 1 << WIDE_BITS;
+// The 12-bit digit that the need-th largest lies in: four bins a lane, sums from the top by wave and over the waves
+__device__ __forceinline__ Digit wide_digit(const uint32_t* hist, uint32_t need) {
+  static_assert(WIDE_BINS == 4 * 1024, "four bins a lane");
+  __shared__ uint32_t totals[16];
+  __shared__ Digit found;
+  const int tid = threadIdx.x, lane = tid & 63;
   uint32_t c[4], sum = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sum += c[i] = hist[4 * lane + i];
-  uint32_t upto = sum; // of this lane and all above it
+  for (int i = 0; i < 4; ++i) sum += c[i] = hist[4 * tid + i];
+  uint32_t upto = sum; // of this lane and all above it in the wave
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const uint32_t v = __shfl_down(upto, o);
     if (lane + o < 64) upto += v;
   }
-  uint32_t above = upto - sum;
-  Digit d{0, 0, 0};
-  bool mine = false;
+  if (lane == 0) totals[tid >> 6] = upto;
+  __syncthreads();
+  for (int w = (tid >> 6) + 1; w < 16; ++w) upto += totals[w];
+  uint32_t over = upto - sum;
+  if (over < need && need <= upto) { // one lane of the workgroup
 #pragma unroll
-  for (int i = 3; i >= 0; --i) {
-    if (!mine && above < need && need <= above + c[i]) {
-      d = Digit{4 * lane + i, above, c[i]};
-      mine = true;
+    for (int i = 3; i >= 0; --i) {
+      if (over < need && need <= over + c[i]) found = Digit{4 * tid + i, over, c[i]};
+      over += c[i];
     }
-    above += c[i];
   }
-  const int l = __ffsll((unsigned long long)__ballot(mine)) - 1; // need is at least 1 and at most the total: one lane has it
-  d.bin = __builtin_amdgcn_readlane(d.bin, l);
-  d.above = (uint32_t)__builtin_amdgcn_readlane((int)d.above, l);
-  d.count = (uint32_t)__builtin_amdgcn_readlane((int)d.count, l);
-  return d;
+  __syncthreads();
+  return found;
 }
 
-// One workgroup per pool.  The need-th largest weight is found digit by digit (8 bits, a histogram in LDS each), starting at
-// the highest bit in which the weights differ at all and ending as soon as a digit holds exactly what is still needed; a
-// second sweep writes what stays, in order.  HELD: the pool fits the workgroup's registers (16384 candidates).
-template <typename W, bool HELD>
+typedef uint32_t Unit16 __attribute__((ext_vector_type(4)));
+constexpr int PUT = 4; // candidates a lane moves at a time: their loads are in flight together
+// (Those past the end move the first one's row, and do not store it.)  N units of every row in flight.
+template <typename Unit, int N>
+__device__ __forceinline__ void move_part(Unit* dst, const Unit* s0, const Unit* s1, const Unit* s2, const Unit* s3, int n, int64_t step) {
+  Unit u0[N], u1[N], u2[N], u3[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    u0[i] = s0[i];
+    u1[i] = s1[i];
+    u2[i] = s2[i];
+    u3[i] = s3[i];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    dst[i] = u0[i];
+    if (n > 1) dst[step + i] = u1[i];
+    if (n > 2) dst[2 * step + i] = u2[i];
+    if (n > 3) dst[3 * step + i] = u3[i];
+  }
+}
+template <typename Unit>
+__device__ __forceinline__ void move_rows(char* dst, const char* s0, const char* s1, const char* s2, const char* s3, int n, int bytes) {
+  Unit* d = reinterpret_cast<Unit*>(dst);
+  const Unit *r0 = reinterpret_cast<const Unit*>(s0), *r1 = reinterpret_cast<const Unit*>(s1);
+  const Unit *r2 = reinterpret_cast<const Unit*>(s2), *r3 = reinterpret_cast<const Unit*>(s3);
+  const int units = bytes / (int)sizeof(Unit);
+  const int64_t step = (int64_t)1024 * units;
+  int i = 0;
+  for (; i + 4 <= units; i += 4) move_part<Unit, 4>(d + i, r0 + i, r1 + i, r2 + i, r3 + i, n, step);
+  switch (units - i) { // uniform
+    case 3: move_part<Unit, 3>(d + i, r0 + i, r1 + i, r2 + i, r3 + i, n, step); break;
+    case 2: move_part<Unit, 2>(d + i, r0 + i, r1 + i, r2 + i, r3 + i, n, step); break;
+    case 1: move_part<Unit, 1>(d + i, r0 + i, r1 + i, r2 + i, r3 + i, n, step); break;
+    default: break;
+  }
+}
+// candidates j0 + kept[0 .. count) of pool b become those that stay from place pos0 on
+template <typename W>
+__device__ __forceinline__ void put_kept(const EvictArgs& a, int64_t b, int64_t pos0, int64_t j0, const uint16_t* kept, int count) {
+  for (int p0 = threadIdx.x; p0 < count; p0 += PUT * 1024) {
+    const int n = (count - p0 + 1023) / 1024; // of this lane's, at most PUT are moved now
+    const int64_t at = b * a.K + pos0 + p0;
+    const int64_t j_0 = j0 + kept[p0], j_1 = n > 1 ? j0 + kept[p0 + 1024] : j_0;
+    const int64_t j_2 = n > 2 ? j0 + kept[p0 + 2048] : j_0, j_3 = n > 3 ? j0 + kept[p0 + 3072] : j_0;
+    const W* w = static_cast<const W*>(a.weights) + b * a.M;
+    W* out = static_cast<W*>(a.out) + at;
+    const W w0 = w[j_0], w1 = w[j_1], w2 = w[j_2], w3 = w[j_3];
+    a.indices[at] = j_0;
+    out[0] = w0;
+    if (n > 1) a.indices[at + 1024] = j_1, out[1024] = w1;
+    if (n > 2) a.indices[at + 2048] = j_2, out[2048] = w2;
+    if (n > 3) a.indices[at + 3072] = j_3, out[3072] = w3;
+    for (int y = 0; y < a.npay; ++y) {
+      const int64_t bytes = a.pay[y].bytes;
+      const char* s = a.pay[y].src + b * a.M * bytes;
+      const char *s0 = s + j_0 * bytes, *s1 = s + j_1 * bytes, *s2 = s + j_2 * bytes, *s3 = s + j_3 * bytes;
+      char* d = a.pay[y].dst + at * bytes;
+      switch (a.pay[y].unit) {
+        case 16: move_rows<Unit16>(d, s0, s1, s2, s3, n, (int)bytes); break;
+        case 8: move_rows<uint64_t>(d, s0, s1, s2, s3, n, (int)bytes); break;
+        case 4: move_rows<uint32_t>(d, s0, s1, s2, s3, n, (int)bytes); break;
+        default: move_rows<uint8_t>(d, s0, s1, s2, s3, n, (int)bytes); break;
+      }
+    }
+  }
+}
+// places pos of pool b that nothing stays in
+template <typename W>
+__device__ __forceinline__ void put_nothing(const EvictArgs& a, int64_t b, int64_t pos) {
+  const int64_t at = b * a.K + pos;
+  a.indices[at] = -1;
+  static_cast<W*>(a.out)[at] = (W)0;
+  for (int y = 0; y < a.npay; ++y)
+    for (int i = 0; i < a.pay[y].bytes; ++i) a.pay[y].dst[at * a.pay[y].bytes + i] = 0;
+}
+
+// Exclusive sums, in the order (i, wave), of the PER x 16 pairs of counts in LDS, from (g0, e0) on; by wave 0.
+template <int PER>
+__device__ __forceinline__ void exclusive_counts(uint32_t* cnt_g, uint32_t* cnt_e, uint32_t g0, uint32_t e0, int lane) {
+  constexpr int N = (PER * 16 + 63) / 64;
+  uint32_t g[N], e[N], sg = 0, se = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool in = N * lane + i < PER * 16;
+    g[i] = sg;
+    e[i] = se;
+    sg += in ? cnt_g[N * lane + i] : 0;
+    se += in ? cnt_e[N * lane + i] : 0;
+  }
+  uint32_t pg = sg, pe = se;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t vg = __shfl_up(pg, o), ve = __shfl_up(pe, o);
+    if (lane >= o) {
+      pg += vg;
+      pe += ve;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (N * lane + i < PER * 16) {
+      cnt_g[N * lane + i] = g0 + pg - sg + g[i];
+      cnt_e[N * lane + i] = e0 + pe - se + e[i];
+    }
+}
+
+// The candidates of 1024 PER places from j0 on, each lane's as bits g (stays), e (stays if among the first `need` of its
+// kind): to their places, behind the g0 and e0 of the candidates before j0.  Compacted in LDS first, so that the outputs are
+// written side by side.
+template <typename W, int PER>
+__device__ __forceinline__ void put_marked(const EvictArgs& a, int64_t b, int64_t j0, uint32_t g_bits, uint32_t e_bits, uint32_t need, uint32_t g0,
+                                           uint32_t e0, int lane, int wave) {
+  __shared__ uint32_t cnt_g[PER * 16], cnt_e[PER * 16];
+  __shared__ uint16_t kept[PER * 1024];
+  __shared__ int total;
+#pragma unroll 1
+  for (int i = 0; i < PER; ++i) {
+    const uint64_t bg = __ballot((g_bits >> i) & 1), be = __ballot((e_bits >> i) & 1);
+    if (lane == 0) {
+      cnt_g[i * 16 + wave] = (uint32_t)__popcll(bg);
+      cnt_e[i * 16 + wave] = (uint32_t)__popcll(be);
+    }
+  }
+  __syncthreads();
+  if (wave == 0) exclusive_counts<PER>(cnt_g, cnt_e, g0, e0, lane);
+  __syncthreads();
+  const uint32_t base = g0 + (e0 < need ? e0 : need);
+#pragma unroll 1
+  for (int i = 0; i < PER; ++i) {
+    const bool g = (g_bits >> i) & 1, e = (e_bits >> i) & 1;
+    const uint64_t bg = __ballot(g), be = __ballot(e), below = (1ull << lane) - 1;
+    const uint32_t ng = cnt_g[i * 16 + wave] + (uint32_t)__popcll(bg & below);
+    const uint32_t ne = cnt_e[i * 16 + wave] + (uint32_t)__popcll(be & below);
+    const uint32_t at = ng + (ne < need ? ne : need) - base;
+    const bool stays = g || (e && ne < need);
+    if (stays) kept[at] = (uint16_t)(i * 1024 + threadIdx.x);
+    if (i == PER - 1 && threadIdx.x == 1023) total = (int)(at + stays);
+  }
+  __syncthreads();
+  put_kept<W>(a, b, base, j0, kept, total);
+}
+
+// One workgroup per pool of at most 1024 PER candidates.
+template <typename W, int PER>
 __global__ __launch_bounds__(1024) void pool_evict_kernel(EvictArgs a) {
   typedef typename KeyOf<W>::type Key;
-  constexpr int BITS = sizeof(Key) * 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t b = blockIdx.x;
   const W* w = static_cast<const W*>(a.weights) + b * a.M;
-  int64_t L = a.M;
-  if (a.lengths) {
-    L = a.len64 ? static_cast<const int64_t*>(a.lengths)[b * a.ls] : (int64_t)static_cast<const int32_t*>(a.lengths)[b * a.ls];
-    L = L < 0 ? 0 : (L > a.M ? a.M : L);
-  }
-  const int64_t keep = L < a.K ? L : a.K;
-  const int64_t lo_free = L <= a.K ? 0 : a.first, hi_free = L <= a.K ? 0 : L - a.recent; // outside: stays whatever its weight
-  uint32_t need = L <= a.K ? 0u : (uint32_t)(a.K - a.first - a.recent);
-  const int64_t chunks = HELD ? 1 : (L + EVICT_CHUNK - 1) / EVICT_CHUNK;
+  const PoolCut cut = pool_cut(a, b);
+  uint32_t need = cut.need;
 
-  __shared__ uint32_t hist[2][256];
-  __shared__ Key sh_and[16], sh_or[16];
-  __shared__ uint32_t cnt_g[EVICT_PER * 16], cnt_e[EVICT_PER * 16];
-  __shared__ uint32_t run_g, run_e;
+  __shared__ uint32_t bins[WIDE_BINS];
+  __shared__ Key sh_keys[2][16];
 
-  Key key[EVICT_PER];
-  auto load = [&](int64_t chunk) {
+  Key key[PER];
+  uint32_t free_bits = 0, g_bits = 0, e_bits = 0;
 #pragma unroll
-    for (int i = 0; i < EVICT_PER; ++i) {
-      const int64_t j = chunk * EVICT_CHUNK + i * 1024 + tid;
-      key[i] = j < L ? order_key(w[j]) : (Key)0;
-    }
-  };
-  auto is_free = [&](int64_t chunk, int i) {
-    const int64_t j = chunk * EVICT_CHUNK + i * 1024 + tid;
-    return j >= lo_free && j < hi_free;
-  };
-  Key prefix = 0;
-  int shift = BITS; // key >> shift against prefix; at BITS nothing is compared
-  if (HELD) load(0);
+  for (int i = 0; i < PER; ++i) {
+    const int64_t j = i * 1024 + tid;
+    key[i] = j < cut.L ? order_key(w[j]) : (Key)0;
+    const bool fr = j >= cut.lo && j < cut.hi;
+    free_bits |= (uint32_t)fr << i;
+    g_bits |= (uint32_t)(j < cut.L && !fr) << i;
+  }
   if (need > 0) {
     Key all = ~(Key)0, any = 0;
-    for (int64_t ch = 0; ch < chunks; ++ch) {
-      if (!HELD) load(ch);
 #pragma unroll
-      for (int i = 0; i < EVICT_PER; ++i)
-        if (is_free(ch, i)) {
-          all &= key[i];
-          any |= key[i];
-        }
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      all &= __shfl_xor(all, o);
-      any |= __shfl_xor(any, o);
-    }
-    if (lane == 0) {
-      sh_and[wave] = all;
-      sh_or[wave] = any;
-    }
-    if (tid < 256) hist[0][tid] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      all &= sh_and[i];
-      any |= sh_or[i];
-    }
-    const Key diff = all ^ any;
-    shift = diff == 0 ? 0 : BITS - (sizeof(Key) == 8 ? __clzll((long long)diff) : __clz((int)diff));
-    prefix = shift < BITS ? all >> shift : (Key)0; // shift == 0: every weight is the same
-    int flip = 0;
-    while (shift > 0) {
-      const int lo = shift > 8 ? shift - 8 : 0, width = shift - lo;
-      for (int64_t ch = 0; ch < chunks; ++ch) {
-        if (!HELD) load(ch);
-#pragma unroll
-        for (int i = 0; i < EVICT_PER; ++i)
-          if (is_free(ch, i) && (shift >= BITS || (key[i] >> (shift & (BITS - 1))) == prefix))
-            atomicAdd(&hist[flip][(uint32_t)(key[i] >> lo) & ((1u << width) - 1u)], 1u);
+    for (int i = 0; i < PER; ++i)
+      if ((free_bits >> i) & 1) {
+        all &= key[i];
+        any |= key[i];
       }
+    all = block_reduce(all, sh_keys[0], key_and<Key>);
+    any = block_reduce(any, sh_keys[1], key_or<Key>);
+    int shift = bits_of<Key>(all ^ any);
+    Key prefix = above(all, shift); // shift == 0: every weight is the same
+    while (shift > 0) {
+      const int lo = shift > WIDE_BITS ? shift - WIDE_BITS : 0, width = shift - lo;
+      for (int i = tid; i < WIDE_BINS; i += 1024) bins[i] = 0;
       __syncthreads();
-      const Digit d = find_digit(hist[flip], need, lane);
-      flip ^= 1;
-      if (tid < 256) hist[flip][tid] = 0;
-      prefix = (shift >= BITS ? (Key)0 : prefix << width) | (Key)d.bin;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (((free_bits >> i) & 1) && above(key[i], shift) == prefix) atomicAdd(&bins[(uint32_t)(key[i] >> lo) & ((1u << width) - 1u)], 1u);
+      __syncthreads();
+      const Digit d = wide_digit(bins, need);
+      prefix = (prefix << width) | (Key)d.bin; // (a prefix of no bits is 0)
       need -= d.above;
       shift = lo;
-      __syncthreads();
       if (need == d.count) break; // the whole digit stays
     }
-  }
-  // above the prefix: stays; equal to it: the first `need` in order
-  const int64_t base = b * a.K;
-  if (tid == 0) run_g = run_e = 0;
-  __syncthreads();
-  for (int64_t ch = 0; ch < chunks; ++ch) {
-    if (!HELD) load(ch);
-    uint32_t g_bits = 0, e_bits = 0;
 #pragma unroll
-    for (int i = 0; i < EVICT_PER; ++i) {
-      const int64_t j = ch * EVICT_CHUNK + i * 1024 + tid;
-      const bool fr = is_free(ch, i);
-      const Key hi = shift >= BITS ? (Key)0 : key[i] >> (shift & (BITS - 1));
-      const bool g = j < L && (!fr || hi > prefix), e = fr && need > 0 && hi == prefix;
-      const uint64_t bg = __ballot(g), be = __ballot(e);
-      if (lane == 0) {
-        cnt_g[i * 16 + wave] = (uint32_t)__popcll(bg);
-        cnt_e[i * 16 + wave] = (uint32_t)__popcll(be);
-      }
-      g_bits |= (uint32_t)g << i;
-      e_bits |= (uint32_t)e << i;
+    for (int i = 0; i < PER; ++i) {
+      const Key hi = above(key[i], shift);
+      const uint32_t fr = (free_bits >> i) & 1;
+      g_bits |= (fr & (uint32_t)(hi > prefix)) << i;
+      e_bits |= (fr & (uint32_t)(hi == prefix)) << i;
     }
-    __syncthreads();
-    if (wave == 0) { // exclusive sums of the 256 counts, in the order of the candidates
-      uint32_t g4[4], e4[4], sg = 0, se = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        g4[i] = sg;
-        e4[i] = se;
-        sg += cnt_g[4 * lane + i];
-        se += cnt_e[4 * lane + i];
-      }
-      uint32_t pg = sg, pe = se;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t vg = __shfl_up(pg, o), ve = __shfl_up(pe, o);
-        if (lane >= o) {
-          pg += vg;
-          pe += ve;
-        }
-      }
-      const uint32_t og = run_g, oe = run_e;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        cnt_g[4 * lane + i] = og + pg - sg + g4[i];
-        cnt_e[4 * lane + i] = oe + pe - se + e4[i];
-      }
-      if (lane == 63) {
-        run_g = og + pg;
-        run_e = oe + pe;
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < EVICT_PER; ++i) {
-      const bool g = (g_bits >> i) & 1, e = (e_bits >> i) & 1;
-      const uint64_t bg = __ballot(g), be = __ballot(e);
-      const uint64_t below = (1ull << lane) - 1;
-      const uint32_t ng = cnt_g[i * 16 + wave] + (uint32_t)__popcll(bg & below);
-      const uint32_t ne = cnt_e[i * 16 + wave] + (uint32_t)__popcll(be & below);
-      if (g || (e && ne < need)) {
-        const int64_t j = ch * EVICT_CHUNK + i * 1024 + tid;
-        const int64_t pos = base + ng + (ne < need ? ne : need);
-        a.indices[pos] = j;
-        static_cast<W*>(a.out)[pos] = w[j];
-      }
-    }
-    __syncthreads();
   }
-  for (int64_t p = keep + tid; p < a.K; p += 1024) {
-    a.indices[base + p] = -1;
-    static_cast<W*>(a.out)[base + p] = (W)0;
-  }
-  if (tid == 0) a.new_lengths[b] = keep;
+  put_marked<W, PER>(a, b, 0, g_bits, e_bits, need, 0, 0, lane, wave);
+  for (int64_t p = cut.keep + tid; p < a.K; p += 1024) put_nothing<W>(a, b, p);
+  if (tid == 0) a.new_lengths[b] = cut.keep;
 }
 
-// Payload rows of what stayed: `row` bytes each, moved in units of UNIT bytes; zeros where nothing stayed.
+// ---- longer pools: chunks of 4096, five launches ----
+constexpr int CHUNK_PER = 4, CHUNK = 1024 * CHUNK_PER;
+constexpr int MAX_TIED = 1024; // candidates told apart one by one in the last launch
+
+template <typename Key>
+struct EvictState { // per pool; behind it, per chunk: {all, any} of Key, counts above and at the prefix
+  uint32_t hist[2][WIDE_BINS];
+  Key prefix[3];    // after the range, the first and the second histogram
+  int shift[3];
+  uint32_t need[3], count[3]; // still needed of those at the prefix; how many there are
+  uint32_t tied;    // candidates collected
+  Key tied_key[MAX_TIED];
+  uint32_t tied_idx[MAX_TIED];
+};
+template <typename Key>
+struct ChunkState {
+  Key all, any, tied_all, tied_any;
+  uint32_t g, e;
+};
+template <typename Key>
+__host__ __device__ inline int64_t evict_state_bytes(int64_t chunks) {
+  return ((int64_t)sizeof(EvictState<Key>) + 255) / 256 * 256 + (chunks * (int64_t)sizeof(ChunkState<Key>) + 255) / 256 * 256;
+}
+template <typename Key>
+struct EvictView {
+  EvictState<Key>* st;
+  ChunkState<Key>* ch;
+};
+template <typename Key>
+__device__ __forceinline__ EvictView<Key> evict_view(const EvictArgs& a, int64_t b) {
+  char* p = static_cast<char*>(a.ws) + b * evict_state_bytes<Key>(a.chunks);
+  return EvictView<Key>{reinterpret_cast<EvictState<Key>*>(p), reinterpret_cast<ChunkState<Key>*>(p + (sizeof(EvictState<Key>) + 255) / 256 * 256)};
+}
+
+template <typename W>
+struct Chunk {
+  typedef typename KeyOf<W>::type Key;
+  Key key[CHUNK_PER];
+  uint32_t free_bits;
+  __device__ __forceinline__ void load(const EvictArgs& a, const PoolCut& cut, int64_t b, int64_t j0) {
+    const W* w = static_cast<const W*>(a.weights) + b * a.M;
+    free_bits = 0;
+#pragma unroll
+    for (int i = 0; i < CHUNK_PER; ++i) {
+      const int64_t j = j0 + i * 1024 + threadIdx.x;
+      key[i] = j < cut.L ? order_key(w[j]) : (Key)0;
+      free_bits |= (uint32_t)(j >= cut.lo && j < cut.hi) << i;
+    }
+  }
+};
+
+template <typename W>
+__global__ __launch_bounds__(1024) void pool_evict_range_kernel(EvictArgs a) {
+  typedef typename KeyOf<W>::type Key;
+  const int64_t b = blockIdx.y, c = blockIdx.x;
+  const PoolCut cut = pool_cut(a, b);
+  const EvictView<Key> v = evict_view<Key>(a, b);
+  for (int64_t i = c * 1024 + threadIdx.x; i < 2 * WIDE_BINS; i += a.chunks * 1024) (&v.st->hist[0][0])[i] = 0;
+  if (c == 0 && threadIdx.x == 0) v.st->tied = 0;
+  Chunk<W> k;
+  k.load(a, cut, b, c * CHUNK);
+  Key all = ~(Key)0, any = 0;
+#pragma unroll
+  for (int i = 0; i < CHUNK_PER; ++i)
+    if ((k.free_bits >> i) & 1) {
+      all &= k.key[i];
+      any |= k.key[i];
+    }
+  __shared__ Key sh[2][16];
+  all = block_reduce(all, sh[0], key_and<Key>);
+  any = block_reduce(any, sh[1], key_or<Key>);
+  if (threadIdx.x == 0) {
+    v.ch[c].all = all;
+    v.ch[c].any = any;
+  }
+}
+
+// What is known of a pool's prefix before launch LEVEL (1, 2: a histogram; 3: collecting): from the launch before, and written
+// for the next by the first chunk.  Nothing is left to decide where need == 0 or every candidate at the prefix stays.
+template <typename Key>
+struct Prefix {
+  Key prefix;
+  int shift;
+  uint32_t need, count;
+};
+template <typename Key, int LEVEL>
+__device__ __forceinline__ Prefix<Key> advance_prefix(const EvictArgs& a, const EvictView<Key>& v, const PoolCut& cut, Key (*sh_keys)[16]) {
+  Prefix<Key> p;
+  if (LEVEL == 1) {
+    Key all = ~(Key)0, any = 0;
+    for (int64_t i = threadIdx.x; i < a.chunks; i += 1024) {
+      all &= v.ch[i].all;
+      any |= v.ch[i].any;
+    }
+    all = block_reduce(all, sh_keys[0], key_and<Key>);
+    any = block_reduce(any, sh_keys[1], key_or<Key>);
+    p.shift = cut.need > 0 ? bits_of<Key>(all ^ any) : 0;
+    p.prefix = above(all, p.shift);
+    p.need = cut.need;
+    p.count = (uint32_t)(cut.hi - cut.lo);
+  } else {
+    p = Prefix<Key>{v.st->prefix[LEVEL - 2], v.st->shift[LEVEL - 2], v.st->need[LEVEL - 2], v.st->count[LEVEL - 2]};
+    if (p.shift > 0 && p.need > 0 && p.need < p.count) {
+      const int lo = p.shift > WIDE_BITS ? p.shift - WIDE_BITS : 0, width = p.shift - lo;
+      const Digit d = wide_digit(v.st->hist[LEVEL - 2], p.need);
+      p.prefix = (p.prefix << width) | (Key)d.bin;
+      p.shift = lo;
+      p.need -= d.above;
+      p.count = d.count;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    v.st->prefix[LEVEL - 1] = p.prefix;
+    v.st->shift[LEVEL - 1] = p.shift;
+    v.st->need[LEVEL - 1] = p.need;
+    v.st->count[LEVEL - 1] = p.count;
+  }
+  return p;
+}
+
+template <typename W, int LEVEL>
+__global__ __launch_bounds__(1024) void pool_evict_hist_kernel(EvictArgs a) {
+  typedef typename KeyOf<W>::type Key;
+  __shared__ uint32_t bins[WIDE_BINS];
+  __shared__ Key sh_keys[2][16];
+  const int64_t b = blockIdx.y, c = blockIdx.x;
+  const PoolCut cut = pool_cut(a, b);
+  const EvictView<Key> v = evict_view<Key>(a, b);
+  Chunk<W> k;
+  k.load(a, cut, b, c * CHUNK);
+  const Prefix<Key> p = advance_prefix<Key, LEVEL>(a, v, cut, sh_keys);
+  if (p.shift == 0 || p.need == 0 || p.need == p.count) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < WIDE_BINS; i += 1024) bins[i] = 0;
+  __syncthreads();
+  const int lo = p.shift > WIDE_BITS ? p.shift - WIDE_BITS : 0, width = p.shift - lo;
+#pragma unroll
+  for (int i = 0; i < CHUNK_PER; ++i)
+    if (((k.free_bits >> i) & 1) && above(k.key[i], p.shift) == p.prefix) atomicAdd(&bins[(uint32_t)(k.key[i] >> lo) & ((1u << width) - 1u)], 1u);
+  __syncthreads();
+  for (int i = threadIdx.x; i < WIDE_BINS; i += 1024)
+    if (bins[i]) atomicAdd(&v.st->hist[LEVEL - 1][i], bins[i]);
+}
+
+template <typename W>
+__global__ __launch_bounds__(1024) void pool_evict_collect_kernel(EvictArgs a) {
+  typedef typename KeyOf<W>::type Key;
+  __shared__ Key sh_keys[2][16];
+  __shared__ uint32_t sh_cnt[2][16];
+  const int64_t b = blockIdx.y, c = blockIdx.x;
+  const PoolCut cut = pool_cut(a, b);
+  const EvictView<Key> v = evict_view<Key>(a, b);
+  Chunk<W> k;
+  k.load(a, cut, b, c * CHUNK);
+  const Prefix<Key> p = advance_prefix<Key, 3>(a, v, cut, sh_keys);
+  const bool open = p.shift > 0 && p.need > 0 && p.need < p.count;
+  uint32_t g = 0, e = 0;
+  Key all = ~(Key)0, any = 0;
+#pragma unroll
+  for (int i = 0; i < CHUNK_PER; ++i) {
+    const int64_t j = c * CHUNK + i * 1024 + threadIdx.x;
+    const bool fr = (k.free_bits >> i) & 1;
+    const Key hi = above(k.key[i], p.shift);
+    g += j < cut.L && (!fr || (p.need > 0 && hi > p.prefix));
+    if (fr && p.need > 0 && hi == p.prefix) {
+      e += 1;
+      all &= k.key[i];
+      any |= k.key[i];
+      if (open && p.count <= MAX_TIED) { // in no particular order: the last launch ranks them
+        const uint32_t at = atomicAdd(&v.st->tied, 1u);
+        v.st->tied_key[at] = k.key[i];
+        v.st->tied_idx[at] = (uint32_t)j;
+      }
+    }
+  }
+  g = wave_sum(g);
+  e = wave_sum(e);
+  if ((threadIdx.x & 63) == 0) {
+    sh_cnt[0][threadIdx.x >> 6] = g;
+    sh_cnt[1][threadIdx.x >> 6] = e;
+  }
+  all = block_reduce(all, sh_keys[0], key_and<Key>);
+  any = block_reduce(any, sh_keys[1], key_or<Key>);
+  if (threadIdx.x == 0) {
+    g = e = 0;
+    for (int i = 0; i < 16; ++i) {
+      g += sh_cnt[0][i];
+      e += sh_cnt[1][i];
+    }
+    v.ch[c].g = g;
+    v.ch[c].e = e;
+    v.ch[c].tied_all = all;
+    v.ch[c].tied_any = any;
+  }
+}
+
+template <typename W>
+__global__ __launch_bounds__(1024) void pool_evict_put_kernel(EvictArgs a) {
+  typedef typename KeyOf<W>::type Key;
+  __shared__ Key sh_key[MAX_TIED];
+  __shared__ uint32_t sh_idx[MAX_TIED], bins[WIDE_BINS];
+  __shared__ Key sh_keys[2][16];
+  __shared__ uint32_t sh_sum[4][16];
+  __shared__ Key cut_key;
+  __shared__ uint32_t cut_idx;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t b = blockIdx.y, c = blockIdx.x, j0 = c * CHUNK;
+  const PoolCut cut = pool_cut(a, b);
+  const EvictView<Key> v = evict_view<Key>(a, b);
+  Prefix<Key> p{v.st->prefix[2], v.st->shift[2], v.st->need[2], v.st->count[2]};
+  Chunk<W> k;
+  k.load(a, cut, b, j0);
+  // candidates before this chunk that stay, or are at the prefix; whether all at the prefix are the same
+  auto add = [](uint32_t x, uint32_t y) { return x + y; };
+  uint32_t g0 = 0, e0 = 0;
+  Key all = ~(Key)0, any = 0;
+  for (int64_t i = tid; i < a.chunks; i += 1024) {
+    if (i < c) {
+      g0 += v.ch[i].g;
+      e0 += v.ch[i].e;
+    }
+    all &= v.ch[i].tied_all;
+    any |= v.ch[i].tied_any;
+  }
+  g0 = block_reduce(g0, sh_sum[0], add);
+  e0 = block_reduce(e0, sh_sum[1], add);
+  all = block_reduce(all, sh_keys[0], key_and<Key>);
+  any = block_reduce(any, sh_keys[1], key_or<Key>);
+  bool open = p.shift > 0 && p.need > 0 && p.need < p.count;
+  bool by_place = false; // ties are cut at (cut_key, cut_idx) instead of by their number
+  if (open && all == any) {
+    p.shift = 0; // the first `need` of equal weights
+    p.prefix = all;
+    open = false;
+  }
+  if (open && p.count <= MAX_TIED) {
+    if (tid < (int)p.count) {
+      sh_key[tid] = v.st->tied_key[tid];
+      sh_idx[tid] = v.st->tied_idx[tid];
+    }
+    __syncthreads();
+    uint32_t taken_before = 0;
+    if (tid < (int)p.count) {
+      const Key kk = sh_key[tid];
+      const uint32_t ii = sh_idx[tid];
+      uint32_t rank = 0;
+      for (uint32_t q = 0; q < p.count; ++q) rank += sh_key[q] > kk || (sh_key[q] == kk && sh_idx[q] < ii);
+      if (rank == p.need - 1) {
+        cut_key = kk;
+        cut_idx = ii;
+      }
+      taken_before = rank < p.need && (int64_t)ii < j0;
+    }
+    e0 = block_reduce(taken_before, sh_sum[2], add);
+    by_place = true;
+  } else if (open) {
+    // many candidates that agree in 24 bits and differ below: this workgroup goes through the whole pool, 12 bits at a time,
+    // and counts what lies before its chunk.  Slow, and rare: weights closer than one part in 4096 all over the pool
+    const Key group = p.prefix;
+    const int group_shift = p.shift;
+    while (p.shift > 0 && p.need < p.count) {
+      const int lo = p.shift > WIDE_BITS ? p.shift - WIDE_BITS : 0, width = p.shift - lo;
+      __syncthreads();
+      for (int i = tid; i < WIDE_BINS; i += 1024) bins[i] = 0;
+      __syncthreads();
+      for (int64_t q = 0; q < a.chunks; ++q) {
+        Chunk<W> o;
+        o.load(a, cut, b, q * CHUNK);
+#pragma unroll
+        for (int i = 0; i < CHUNK_PER; ++i)
+          if (((o.free_bits >> i) & 1) && above(o.key[i], p.shift) == p.prefix) atomicAdd(&bins[(uint32_t)(o.key[i] >> lo) & ((1u << width) - 1u)], 1u);
+      }
+      __syncthreads();
+      const Digit d = wide_digit(bins, p.need);
+      p.prefix = (p.prefix << width) | (Key)d.bin;
+      p.shift = lo;
+      p.need -= d.above;
+      p.count = d.count;
+    }
+    uint32_t more = 0, same = 0; // of the group, before this chunk: above the new prefix, at it
+    for (int64_t q = 0; q < c; ++q) {
+      Chunk<W> o;
+      o.load(a, cut, b, q * CHUNK);
+#pragma unroll
+      for (int i = 0; i < CHUNK_PER; ++i)
+        if (((o.free_bits >> i) & 1) && above(o.key[i], group_shift) == group) {
+          more += above(o.key[i], p.shift) > p.prefix;
+          same += above(o.key[i], p.shift) == p.prefix;
+        }
+    }
+    g0 += block_reduce(more, sh_sum[2], add);
+    e0 = block_reduce(same, sh_sum[3], add);
+  }
+  uint32_t g_bits = 0, e_bits = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < CHUNK_PER; ++i) {
+    const int64_t j = j0 + i * 1024 + tid;
+    const bool fr = (k.free_bits >> i) & 1;
+    const Key hi = above(k.key[i], p.shift);
+    g_bits |= (uint32_t)(j < cut.L && (!fr || (p.need > 0 && hi > p.prefix))) << i;
+    bool e = fr && p.need > 0 && hi == p.prefix;
+    if (by_place) e = e && (k.key[i] > cut_key || (k.key[i] == cut_key && (uint32_t)j <= cut_idx));
+    e_bits |= (uint32_t)e << i;
+  }
+  put_marked<W, CHUNK_PER>(a, b, j0, g_bits, e_bits, p.need, g0, e0, lane, wave);
+  for (int64_t q = cut.keep + c * 1024 + tid; q < a.K; q += a.chunks * 1024) put_nothing<W>(a, b, q);
+  if (c == 0 && tid == 0) a.new_lengths[b] = cut.keep;
+}
+
+// Payload rows too long for that: `row` bytes each, moved in units; zeros where nothing stayed.
 template <typename Unit>
 __global__ __launch_bounds__(256) void pool_gather_kernel(const int64_t* indices, const Unit* src, Unit* dst, int64_t total, int64_t K, int64_t M, int units) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
@@ -441,9 +878,6 @@ __global__ __launch_bounds__(256) void pool_gather_kernel(const int64_t* indices
     dst[i] = v;
   }
 }
-struct alignas(16) Unit16 {
-  uint32_t v[4];
-};
 template <typename Unit>
 void gather_launch(const int64_t* indices, const void* src, void* dst, int64_t pools, int64_t K, int64_t M, int64_t row_bytes, hipStream_t st) {
   const int64_t units = row_bytes / (int64_t)sizeof(Unit), total = pools * K * units;
@@ -471,7 +905,7 @@ WeightPlan weight_plan(int64_t pools, int64_t R, int64_t M, int dtype) {
 }
 int column_groups(int64_t pools, int64_t R, int64_t M, int vec) {
   const int64_t tiles = (M + 256 * vec - 1) / (256 * vec) * (pools > 0 ? pools : 1);
-  int64_t g = (512 + tiles - 1) / tiles; // workgroups that keep the memory busy
+  int64_t g = (1024 + tiles - 1) / tiles; // workgroups that keep the memory busy
   const int64_t most = (R + 15) / 16;
   g = g > most ? most : g;
   return (int)(g < 1 ? 1 : (g > 64 ? 64 : g));
@@ -513,9 +947,46 @@ void weights_launch(const WeightArgs& a, const WeightPlan& p, int64_t pools, hip
   if (a.groups > 1) hipLaunchKernelGGL(pool_weights_join_kernel<A>, dim3((a.sc.M + 63) / 64, (unsigned)pools), dim3(256), 0, st, a);
 }
 
+// the widest access that a payload's rows allow on both sides
+int payload_unit(const void* src, const void* dst, int64_t row_bytes) {
+  const uintptr_t al = (uintptr_t)src | (uintptr_t)dst | (uintptr_t)row_bytes;
+  return al % 16 == 0 ? 16 : al % 8 == 0 ? 8 : al % 4 == 0 ? 4 : al % 2 == 0 ? 2 : 1;
+}
+constexpr int64_t HELD_MAX = 16 * 1024; // candidates that one workgroup holds in its registers
+int64_t evict_workspace(int dtype, int64_t pools, int64_t M) {
+  if (M <= HELD_MAX) return 0;
+  const int64_t chunks = (M + CHUNK - 1) / CHUNK;
+  return pools * (dtype == GPX_DTYPE_F64 ? evict_state_bytes<uint64_t>(chunks) : evict_state_bytes<uint32_t>(chunks));
+}
+template <typename W>
+void evict_launch(const EvictArgs& a, int64_t pools, hipStream_t st) {
+  const dim3 block(1024);
+  if (a.M <= HELD_MAX) {
+    const dim3 grid((unsigned)pools);
+    if (a.M <= 1024)
+      hipLaunchKernelGGL((pool_evict_kernel<W, 1>), grid, block, 0, st, a);
+    else if (a.M <= 4096)
+      hipLaunchKernelGGL((pool_evict_kernel<W, 4>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((pool_evict_kernel<W, 16>), grid, block, 0, st, a);
+    return;
+  }
+  const dim3 grid((unsigned)a.chunks, (unsigned)pools);
+  hipLaunchKernelGGL(pool_evict_range_kernel<W>, grid, block, 0, st, a);
+  hipLaunchKernelGGL((pool_evict_hist_kernel<W, 1>), grid, block, 0, st, a);
+  hipLaunchKernelGGL((pool_evict_hist_kernel<W, 2>), grid, block, 0, st, a);
+  hipLaunchKernelGGL(pool_evict_collect_kernel<W>, grid, block, 0, st, a);
+  hipLaunchKernelGGL(pool_evict_put_kernel<W>, grid, block, 0, st, a);
+}
+
 } // namespace
 
 extern "C" {
+
+int64_t gpx_pool_evict_workspace(int64_t pools, int64_t candidates, int dtype) {
+  if (pools < 0 || candidates < 0 || (dtype != GPX_DTYPE_F64 && dtype != GPX_DTYPE_F32)) return -1;
+  return evict_workspace(dtype, pools, candidates);
+}
 
 int64_t gpx_pool_weights_workspace(int64_t pools, int64_t rows, int64_t candidates, int dtype) {
   if (pools < 0 || rows < 0 || candidates < 0 || dtype < GPX_DTYPE_F64 || dtype > GPX_DTYPE_F16) return -1;
@@ -560,10 +1031,11 @@ int gpx_pool_weights(gpx_ctx* ctx, const gpx_scores* scores, const void* d_row_w
 int gpx_pool_evict(gpx_ctx* ctx, int dtype, int64_t pools, int64_t candidates, const void* d_weights, const void* d_lengths,
                    int lengths_64, int64_t lengths_stride, int64_t budget, int64_t first, int64_t recent, int64_t* d_indices,
                    int64_t* d_new_lengths, void* d_weights_out, int npayload, const void* const* d_payload,
-                   void* const* d_payload_out, const int64_t* payload_row_bytes, void* stream) {
+                   void* const* d_payload_out, const int64_t* payload_row_bytes, void* d_workspace, int64_t workspace_bytes,
+                   void* stream) {
   if (!ctx || ctx->device < 0) return -1;
   if (dtype != GPX_DTYPE_F64 && dtype != GPX_DTYPE_F32) return bad_arg(ctx, "gpx_pool_evict: weights are float64 or float32");
-  if (pools < 0 || candidates < 0 || pools > INT32_MAX / 1024 / 4 || candidates > INT32_MAX - 65536)
+  if (pools < 0 || candidates < 0 || pools > 65535 || candidates > INT32_MAX - 65536)
     return bad_arg(ctx, "gpx_pool_evict: sizes");
   if (budget < 1 || budget > INT32_MAX) return bad_arg(ctx, "gpx_pool_evict: the budget must be positive");
   if (first < 0 || recent < 0 || first + recent > budget) return bad_arg(ctx, "gpx_pool_evict: first + recent exceed the budget");
@@ -574,37 +1046,45 @@ int gpx_pool_evict(gpx_ctx* ctx, int dtype, int64_t pools, int64_t candidates, c
     if (payload_row_bytes[i] < 0 || payload_row_bytes[i] > INT32_MAX) return bad_arg(ctx, "gpx_pool_evict: payload row size");
     if (payload_row_bytes[i] > 0 && ((!d_payload[i] && candidates > 0) || !d_payload_out[i])) return bad_arg(ctx, "gpx_pool_evict: null payload");
   }
-  EvictArgs a{d_weights, d_lengths, lengths_64, lengths_stride, candidates, budget, first, recent, d_indices, d_new_lengths, d_weights_out};
+  EvictArgs a{};
+  a.weights = d_weights;
+  a.lengths = d_lengths;
+  a.len64 = lengths_64;
+  a.ls = lengths_stride;
+  a.M = candidates;
+  a.K = budget;
+  a.first = first;
+  a.recent = recent;
+  a.indices = d_indices;
+  a.new_lengths = d_new_lengths;
+  a.out = d_weights_out;
+  a.ws = d_workspace;
+  a.chunks = (candidates + CHUNK - 1) / CHUNK;
+  for (int i = 0; i < npayload; ++i) {
+    const int64_t rb = payload_row_bytes[i];
+    if (rb == 0 || rb > FUSED_ROW_BYTES) continue;
+    const int unit = payload_unit(d_payload[i], d_payload_out[i], rb);
+    a.pay[a.npay++] = Payload{static_cast<const char*>(d_payload[i]), static_cast<char*>(d_payload_out[i]), (int)rb, unit == 2 ? 1 : unit};
+  }
+  const int64_t need = evict_workspace(dtype, pools, candidates);
+  if (need > 0 && (!d_workspace || workspace_bytes < need)) return bad_arg(ctx, "gpx_pool_evict: workspace too small (gpx_pool_evict_workspace)");
   DeviceGuard g(ctx->device);
   GPX_HIP(ctx, g.err);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)pools), block(1024);
-  const bool held = candidates <= EVICT_CHUNK;
-  if (dtype == GPX_DTYPE_F64) {
-    if (held)
-      hipLaunchKernelGGL((pool_evict_kernel<double, true>), grid, block, 0, st, a);
-    else
-      hipLaunchKernelGGL((pool_evict_kernel<double, false>), grid, block, 0, st, a);
-  } else {
-    if (held)
-      hipLaunchKernelGGL((pool_evict_kernel<float, true>), grid, block, 0, st, a);
-    else
-      hipLaunchKernelGGL((pool_evict_kernel<float, false>), grid, block, 0, st, a);
-  }
+  if (dtype == GPX_DTYPE_F64)
+    evict_launch<double>(a, pools, st);
+  else
+    evict_launch<float>(a, pools, st);
   for (int i = 0; i < npayload; ++i) {
     const int64_t rb = payload_row_bytes[i];
-    if (rb == 0) continue;
-    const uintptr_t al = (uintptr_t)d_payload[i] | (uintptr_t)d_payload_out[i] | (uintptr_t)rb;
-    if (al % 16 == 0)
-      gather_launch<Unit16>(d_indices, d_payload[i], d_payload_out[i], pools, budget, candidates, rb, st);
-    else if (al % 8 == 0)
-      gather_launch<uint64_t>(d_indices, d_payload[i], d_payload_out[i], pools, budget, candidates, rb, st);
-    else if (al % 4 == 0)
-      gather_launch<uint32_t>(d_indices, d_payload[i], d_payload_out[i], pools, budget, candidates, rb, st);
-    else if (al % 2 == 0)
-      gather_launch<uint16_t>(d_indices, d_payload[i], d_payload_out[i], pools, budget, candidates, rb, st);
-    else
-      gather_launch<uint8_t>(d_indices, d_payload[i], d_payload_out[i], pools, budget, candidates, rb, st);
+    if (rb <= FUSED_ROW_BYTES) continue;
+    switch (payload_unit(d_payload[i], d_payload_out[i], rb)) {
+      case 16: gather_launch<Unit16>(d_indices, d_payload[i], d_payload_out[i], pools, budget, candidates, rb, st); break;
+      case 8: gather_launch<uint64_t>(d_indices, d_payload[i], d_payload_out[i], pools, budget, candidates, rb, st); break;
+      case 4: gather_launch<uint32_t>(d_indices, d_payload[i], d_payload_out[i], pools, budget, candidates, rb, st); break;
+      case 2: gather_launch<uint16_t>(d_indices, d_payload[i], d_payload_out[i], pools, budget, candidates, rb, st); break;
+      default: gather_launch<uint8_t>(d_indices, d_payload[i], d_payload_out[i], pools, budget, candidates, rb, st); break;
+    }
   }
   GPX_HIP(ctx, hipGetLastError());
   return 0;

@@ -444,10 +444,12 @@ int gpx_pool_weights(gpx_ctx* ctx, const gpx_scores* scores, const void* d_row_w
  * new_lengths, weights, and the rows of up to 16 payload arrays (pools x candidates x payload_row_bytes, contiguous) are
  * written to the outputs, with zeros behind the last.  The arrays of payload pointers are host arrays; outputs must not
  * overlap inputs. */
+int64_t gpx_pool_evict_workspace(int64_t pools, int64_t candidates, int dtype);
 int gpx_pool_evict(gpx_ctx* ctx, int dtype, int64_t pools, int64_t candidates, const void* d_weights, const void* d_lengths,
                    int lengths_64, int64_t lengths_stride, int64_t budget, int64_t first, int64_t recent, int64_t* d_indices,
                    int64_t* d_new_lengths, void* d_weights_out, int npayload, const void* const* d_payload,
-                   void* const* d_payload_out, const int64_t* payload_row_bytes, void* stream);
+                   void* const* d_payload_out, const int64_t* payload_row_bytes, void* d_workspace,
+                   int64_t workspace_bytes, void* stream);
 /* Staging of host arrays for the above: scratch of the context (valid until the next gpx_scratch, which waits for the
  * context's stream), blocking copies, and that stream. */
 int gpx_scratch(gpx_ctx* ctx, int64_t bytes, void** d_out);

@@ -84,7 +84,7 @@ class PoolEngine(OracleEngine):
         view(out, acc, (shape[0], shape[2]))[...] = ref.weights(x, w, decay, u, T, mask, lengths)
 
     def pool_evict(self, dtype, pools, candidates, weights, lengths, lengths_64, lengths_stride, budget, first, recent, indices,
-                   new_lengths, weights_out, payload, payload_out, row_bytes, stream):
+                   new_lengths, weights_out, payload, payload_out, row_bytes, workspace, workspace_bytes, stream):
         w = view(weights, KIND[dtype], (pools, candidates))
         n = view(lengths, "int64" if lengths_64 else "int32", (pools,), [lengths_stride]) if lengths else None
         pay = [view(p, "uint8", (pools, candidates, b)) for p, b in zip(payload, row_bytes)]

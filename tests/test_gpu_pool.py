@@ -245,7 +245,7 @@ def check_evict(w, budget, payload=(), **kw):
 
 
 E_SHAPES = [((1,), 1), ((7,), 3), ((201,), 50), ((64,), 64), ((65,), 100), ((4, 1023), 1), ((3, 1025), 1024), ((5, 16384), 4096),
-            ((2, 16385), 5000), ((1, 100003), 33333), ((2, 0), 4), ((0, 5), 2), ((300, 40), 17)]
+            ((2, 16385), 5000), ((1, 100003), 33333), ((3, 20480), 2047), ((2, 0), 4), ((0, 5), 2), ((300, 40), 17)]
 
 
 @pytest.mark.parametrize("kind", ["float64", "float32"])
@@ -346,7 +346,7 @@ def test_a_step_is_captured_and_replayed():
         e = acq.pool_evict(w, 3000, (pts,), recent=5)
         v = acq.pool_weights(small)
         d = acq.pool_evict(v, 100)
-        return [*r[:5], r.stats, g, w, e.indices, e.lengths, e.weights, e.payload[0], v, d.indices, d.weights]
+        return [*r, g, w, e.indices, e.lengths, e.weights, e.payload[0], v, d.indices, d.weights]
 
     step()
     torch.cuda.synchronize()
@@ -439,4 +439,6 @@ def test_the_library_refuses_what_the_kernels_do_not_take():
     with pytest.raises(_lib.GpxError):  # needs a workspace
         eng.choice_logprobs(long, 0, 0, 0, 1, 1, 1, 1, 1, 1, 0, 0, 0)
     with pytest.raises(_lib.GpxError):
-        eng.pool_evict(0, 1, 8, 0, 0, False, 0, 4, 0, 0, 1, 1, 1, [], [], [], 0)
+        eng.pool_evict(0, 1, 8, 0, 0, False, 0, 4, 0, 0, 1, 1, 1, [], [], [], 0, 0, 0)
+    with pytest.raises(_lib.GpxError):  # needs a workspace
+        eng.pool_evict(0, 1, 1 << 20, 1, 0, False, 0, 4, 0, 0, 1, 1, 1, [], [], [], 0, 0, 0)
