@@ -26,6 +26,7 @@ from .. import _lib
 
 MAX_TOP = 64
 MAX_PAYLOAD = 16
+_MAX_POOL = (1 << 31) - 1 - (1 << 20)
 _DTYPES = {"float64": 0, "float32": 1, "bfloat16": 2, "float16": 3}
 _INTS = ("int64", "int32")
 _MASKS = ("bool", "uint8")
@@ -239,8 +240,8 @@ class _Policy:
         self.pools, self.rows = p, r = lead if len(lead) == 2 else (1, lead[0]) if lead else (1, 1)
         if p * r > 1 << 25:
             raise ValueError("more than 2^25 rows of scores")
-        if M > (1 << 31) - 1 - 65536:
-            raise ValueError("more than 2^31 - 65537 candidates")
+        if M > _MAX_POOL:
+            raise ValueError("more than 2^31 - 2^20 candidates")
         self.mask = self.lengths = self.temps = None
         ms, ls, ts = (0, 0, 0), (0, 0), (0, 0)
         n64 = 0
@@ -483,8 +484,8 @@ def pool_evict(weights, budget: int, payload: Sequence = (), *, first: int = 0, 
         raise ValueError(f"the budget is {budget}; expected a positive number")
     if first < 0 or recent < 0 or first + recent > budget:
         raise ValueError(f"first = {first} and recent = {recent} must not be negative, and together at most the budget {budget}")
-    if pools > 65535 or M > (1 << 31) - 1 - 65536:
-        raise ValueError("more than 65535 pools, or 2^31 - 65537 candidates")
+    if pools > 65535 or M > _MAX_POOL:
+        raise ValueError("more than 65535 pools, or 2^31 - 2^20 candidates")
     n, n_stride, n64 = None, 0, False
     if lengths is not None:
         n = sp.take(lengths, "lengths", _INTS)

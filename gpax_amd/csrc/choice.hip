@@ -30,6 +30,13 @@ struct ChoiceArgs {
   void* ws;
 };
 
+// The kernel's arguments as if read from memory here: hides from the compiler that they are the ones it has already.
+__device__ __forceinline__ const ChoiceArgs& late_args(const ChoiceArgs&) {
+  uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const ChoiceArgs*)(const __attribute__((address_space(4))) ChoiceArgs*)p;
+}
+
 // A partial result in the workspace: statistics and the list, of one split of one row
 template <typename A>
 struct Partial {
@@ -49,30 +56,36 @@ __device__ __forceinline__ bool before(A k1, uint32_t i1, A k2, uint32_t i2) {
 }
 
 // Bitonic networks over the 64 lanes, best first, unrolled: the stage (SIZE, STRIDE) and all behind it.  From (2, 1) on it
-// sorts; from (64, 32) on it sorts what is a bitonic sequence already.
-template <int SIZE, int STRIDE, typename A>
-__device__ __forceinline__ void bitonic(A& k, uint32_t& i, int lane) {
-  const A ok = xor_lane<STRIDE>(k);
-  const uint32_t oi = xor_lane<STRIDE>(i);
-  const bool keep_first = ((lane & STRIDE) == 0) == ((lane & SIZE) == 0);
-  if (before(k, i, ok, oi) != keep_first) {
-    k = ok;
-    i = oi;
-  }
-  if constexpr (STRIDE > 1)
-    bitonic<SIZE, STRIDE / 2>(k, i, lane);
-  else if constexpr (SIZE < 64)
-    bitonic<SIZE * 2, SIZE>(k, i, lane);
+// sorts; from (64, 32) on it sorts what is a bitonic sequence already.  Which lanes keep the better one is a constant of the
+// stage: as a literal in the scalar unit it costs no register (21 such masks, kept in registers, spilled).
+constexpr uint64_t keep_better(int size, int stride) {
+  uint64_t m = 0;
+  for (int l = 0; l < 64; ++l)
+    if (((l & stride) == 0) == ((l & size) == 0)) m |= (uint64_t)1 << l;
+  return m;
 }
 template <int SIZE, int STRIDE, typename A>
-__device__ __forceinline__ void bitonic_values(A& v, int lane) {
-  const A o = xor_lane<STRIDE>(v);
-  const bool keep_first = ((lane & STRIDE) == 0) == ((lane & SIZE) == 0);
-  v = (v > o) == keep_first ? v : o;
+__device__ __forceinline__ void bitonic(A& k, uint32_t& i) {
+  constexpr uint64_t KEEP = keep_better(SIZE, STRIDE);
+  const A ok = xor_lane<STRIDE>(k);
+  const uint32_t oi = xor_lane<STRIDE>(i);
+  const bool swap = __builtin_amdgcn_inverse_ballot_w64(__ballot(before(k, i, ok, oi)) ^ KEEP);
+  k = swap ? ok : k;
+  i = swap ? oi : i;
   if constexpr (STRIDE > 1)
-    bitonic_values<SIZE, STRIDE / 2>(v, lane);
+    bitonic<SIZE, STRIDE / 2>(k, i);
   else if constexpr (SIZE < 64)
-    bitonic_values<SIZE * 2, SIZE>(v, lane);
+    bitonic<SIZE * 2, SIZE>(k, i);
+}
+template <int SIZE, int STRIDE, typename A>
+__device__ __forceinline__ void bitonic_values(A& v) {
+  constexpr uint64_t KEEP = keep_better(SIZE, STRIDE);
+  const A o = xor_lane<STRIDE>(v);
+  v = __builtin_amdgcn_inverse_ballot_w64(__ballot(v > o) ^ KEEP) ? o : v;
+  if constexpr (STRIDE > 1)
+    bitonic_values<SIZE, STRIDE / 2>(v);
+  else if constexpr (SIZE < 64)
+    bitonic_values<SIZE * 2, SIZE>(v);
 }
 
 template <typename A>
@@ -101,7 +114,7 @@ struct TopList {
       key = rk;
       idx = ri;
     }
-    bitonic<64, 32>(key, idx, lane);
+    bitonic<64, 32>(key, idx);
     rethreshold();
   }
   // one candidate a lane (those that do not pass the threshold are dropped)
@@ -112,7 +125,13 @@ struct TopList {
     if (__popcll(in) > INSERT_MAX) {
       A ck = pass ? x : neg_inf<A>();
       uint32_t ci = pass ? j : 0xffffffffu;
-      bitonic<2, 1>(ck, ci, lane);
+      bitonic<2, 1>(ck, ci);
+      if (read_lane(idx, 0) == 0xffffffffu) { // the first ones
+        key = ck;
+        idx = ci;
+        rethreshold();
+        return;
+      }
       merge_sorted(ck, ci, lane);
       return;
     }
@@ -139,15 +158,21 @@ struct TopList {
   }
 };
 
-// The candidates of a step that may belong into the list.  Only those at or above a bound are looked at one by one: the list's
-// threshold, or, where at least k lanes hold something better, the k-th largest of the lanes' maxima (k candidates reach it, so
-// no other can be among the best k).  What passes is kept in LDS by its index and waits there until 64 are together, or the
-// row ends; then the scores are read again, from the cache, and offered 64 at a time.  A threshold that is not up to date only
-// lets more pass.
+// The candidates that may belong into the list.  Of a step only those at or above a bound are looked at one by one: the list's
+// threshold, the threshold of all waves of the row, or, where many lanes (and at least k) hold something better, the k-th
+// largest of the lanes' maxima (k candidates reach it, so no other can be among the best k).  What passes waits in LDS until 64
+// are together or the waves compare notes; it is offered 64 at a time, the first 64 with their scores, more than that by their
+// index, and those scores are read again from the cache.  A threshold that is not up to date only lets more pass.
+template <typename A, int E>
+struct WaitingRoom {
+  A keys[64];
+  uint32_t idx[64 * E + 64];
+};
 template <typename T, int VEC, int U>
 struct Waiting {
   typedef typename Acc<T>::type A;
-  uint32_t* idx; // U * VEC * 64 + 64 of this wave
+  WaitingRoom<A, U * VEC>& room; // this wave's
+  A shared;                      // k candidates of the row reach it
   int count;
 
   __device__ __forceinline__ void flush(TopList<A>& list, const Row<T>& v, int lane) {
@@ -157,40 +182,70 @@ struct Waiting {
       A k = neg_inf<A>();
       uint32_t j = 0xffffffffu;
       if (i + lane < count) {
-        j = idx[i + lane];
-        k = to_acc(v.x[j * v.xc]);
+        j = room.idx[i + lane];
+        if (i == 0)
+          k = room.keys[lane];
+        else
+          k = to_acc(v.x[j * v.xc]);
       }
       list.consume(k, j, lane);
     }
     __builtin_amdgcn_wave_barrier();
     count = 0;
   }
-  // a step; true: 64 or more wait
-  __device__ __forceinline__ bool step(const TopList<A>& list, const A* x, A cm, int64_t j0, int lane) {
-    // strictly above: a score equal to the k-th loses to it, whose index is lower (a wave takes its steps in order)
-    const uint64_t better = __ballot(cm > list.thr_key);
-    if (better == 0) return false;
-    A bound = list.thr_key;
-    bool strict = true;
-    if (__popcll(better) >= list.k) {
-      bound = cm;
-      bitonic_values<2, 1>(bound, lane);
-      bound = read_lane(bound, list.k - 1);
-      strict = false;
+  __device__ __forceinline__ void step(TopList<A>& list, const Row<T>& v, const A* x, A cm, int j0, int lane) {
+    // above the list's own threshold strictly: a score equal to its k-th loses to it, whose index is lower (a wave takes its
+    // steps in order); at or above the shared one, whose index may be anything
+    const A own = list.thr_key;
+    const uint64_t better = __ballot(cm > own && cm >= shared);
+    if (better == 0) return;
+    A bound = shared;
+    const bool many = __popcll(better) >= (list.k > 32 ? list.k : 32);
+    if (many) {
+      A sorted = cm;
+      bitonic_values<2, 1>(sorted);
+      const A kth = read_lane(sorted, list.k - 1);
+      bound = kth > bound ? kth : bound;
     }
 #pragma unroll
     for (int e = 0; e < U * VEC; ++e) {
-      const bool in = strict ? x[e] > bound : x[e] >= bound && x[e] > list.thr_key;
+      const bool in = x[e] > own && x[e] >= bound;
       const uint64_t mask = __ballot(in);
       if (mask) {
         const int at = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
-        if (in) idx[at] = (uint32_t)(j0 + (e / VEC) * 64 * VEC + lane * VEC + e % VEC);
+        if (in) {
+          room.idx[at] = (uint32_t)(j0 + (e / VEC) * 64 * VEC + lane * VEC + e % VEC);
+          if (at < 64) room.keys[at] = x[e];
+        }
         count += __popcll(mask);
       }
     }
-    return count >= 64 || !strict; // with a bound of its own the step has much for the list: the threshold comes next
+    if (many || count >= 64) flush(list, v, lane); // (many: the threshold will be much better)
   }
 };
+
+// What the waves of a workgroup tell each other: statistics, and their lists in the front of their waiting rooms, which are
+// empty then (LDS decides how many workgroups a CU holds).
+template <typename A, int W>
+struct WaveShare {
+  Stats<A> st[W];
+  A thr;
+};
+// The k-th best of all waves' candidates so far.  Lists stay with their waves.
+template <typename A, int W, int E>
+__device__ __forceinline__ A common_threshold(const TopList<A>& list, WaitingRoom<A, E>* rooms, WaveShare<A, W>& sh, int wave, int lane) {
+  rooms[wave].keys[lane] = list.key;
+  rooms[wave].idx[lane] = list.idx;
+  __syncthreads();
+  if (wave == 0) {
+    TopList<A> all = list;
+#pragma unroll 1
+    for (int w = 1; w < W; ++w) all.consume_sorted(rooms[w].keys[lane], rooms[w].idx[lane], lane);
+    if (lane == 0) sh.thr = all.thr_key;
+  }
+  __syncthreads();
+  return sh.thr;
+}
 
 // What a row's statistics are turned into, by a team of `size` threads of which this one is `at`; the list by its wave.
 template <typename T>
@@ -231,24 +286,21 @@ __device__ __forceinline__ void finish_top(const ChoiceArgs& a, int64_t row, int
 }
 
 // Joins the statistics and lists of the W waves of a workgroup: log2 W rounds, each wave with the one `half` above it.
-template <typename A, int W, bool TOP>
-__device__ __forceinline__ void join_waves(Stats<A>& st, TopList<A>& list, A c, int wave, int lane) {
-  __shared__ Stats<A> sh_st[W];
-  __shared__ A sh_key[TOP ? W : 1][64];
-  __shared__ uint32_t sh_idx[TOP ? W : 1][64];
+template <typename A, int W, bool TOP, int E>
+__device__ __forceinline__ void join_waves(Stats<A>& st, TopList<A>& list, A c, WaitingRoom<A, E>* rooms, WaveShare<A, W>& sh, int wave, int lane) {
 #pragma unroll 1
   for (int half = W / 2; half > 0; half >>= 1) {
     if (wave >= half && wave < 2 * half) {
-      if (lane == 0) sh_st[wave] = st;
+      if (lane == 0) sh.st[wave] = st;
       if (TOP) {
-        sh_key[wave][lane] = list.key;
-        sh_idx[wave][lane] = list.idx;
+        rooms[wave].keys[lane] = list.key;
+        rooms[wave].idx[lane] = list.idx;
       }
     }
     __syncthreads();
     if (wave < half) {
-      st = stats_join(st, sh_st[wave + half], c);
-      if (TOP) list.consume_sorted(sh_key[wave + half][lane], sh_idx[wave + half][lane], lane);
+      st = stats_join(st, sh.st[wave + half], c);
+      if (TOP) list.consume_sorted(rooms[wave + half].keys[lane], rooms[wave + half].idx[lane], lane);
     }
   }
 }
@@ -261,10 +313,11 @@ struct StepOf {
 };
 
 template <typename T, int WAVES, bool TOP, int U>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void choice_rows_kernel(ChoiceArgs a) {
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, sizeof(T) == 8 || WAVES != 4 ? 1 : 8) void choice_rows_kernel(ChoiceArgs a) {
   typedef typename Acc<T>::type A;
   constexpr int VEC = VecOf<T>::value;
-  __shared__ uint32_t sh_waiting[TOP ? (WAVES == 1 ? 4 : WAVES) : 1][TOP ? U * VEC * 64 + 64 : 1];
+  __shared__ WaitingRoom<A, U * VEC> sh_room[TOP ? (WAVES == 1 ? 4 : WAVES) : 1];
+  __shared__ WaveShare<A, WAVES> sh_share;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
   if (row >= a.sc.rows) return; // WAVES == 1: whole waves, and no barrier below
@@ -274,40 +327,54 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void choice_rows_ker
   Stats<A> st = stats_empty<A>();
   TopList<A> list;
   if (TOP) list.init(a.top);
-  Waiting<T, VEC, U> waiting{sh_waiting[wave], 0};
-  const int64_t step = (int64_t)64 * VEC * U;
-  const int64_t first = WAVES == 1 ? 0 : ((int64_t)blockIdx.y * WAVES + wave) * step;
-  const int64_t stride = WAVES == 1 ? step : (int64_t)a.splits * WAVES * step;
-  for (int64_t j0 = first; j0 < v.n; j0 += stride) {
-    A x[U * VEC];
-    load_step<T, VEC, U>(v, j0, 64 * VEC, lane * VEC, x);
-    A cm = x[0];
+  // candidates are numbered in 32 bits: a pool ends 2^20 short of 2^31, and no stride (2^18 at most) is longer than that
+  const int step = 64 * VEC * U;
+  const int first = WAVES == 1 ? 0 : ((int)blockIdx.y * WAVES + wave) * step;
+  const int stride = WAVES == 1 ? step : a.splits * WAVES * step;
+  const int steps = (int)(((uint32_t)v.n + (uint32_t)stride - 1) / (uint32_t)stride); // the same for all waves of the row's workgroup: they meet at barriers
+  Waiting<T, VEC, U> waiting{sh_room[TOP ? wave : 0], neg_inf<A>(), 0};
+  for (int i = 0; i < steps; ++i) {
+    const int j0 = first + i * stride;
+    if (j0 < v.n) {
+      A x[U * VEC];
+      load_step<T, VEC, U>(v, j0, 64 * VEC, lane * VEC, x);
+      A cm = x[0];
 #pragma unroll
-    for (int e = 1; e < U * VEC; ++e) cm = fmax(cm, x[e]);
-    stats_add<A, U * VEC>(st, x, cm, c);
-    if constexpr (TOP) {
-      if (waiting.step(list, x, cm, j0, lane)) waiting.flush(list, v, lane);
+      for (int e = 1; e < U * VEC; ++e) cm = fmax(cm, x[e]);
+      stats_add<A, U * VEC>(st, x, cm, c);
+      if constexpr (TOP) waiting.step(list, v, x, cm, j0, lane);
+    }
+    if constexpr (TOP && WAVES > 1) {
+      // a threshold of the whole row after 1, 2, 4 ... steps: between two of them about k candidates of the row pass it
+      if (i + 1 < steps && ((i + 1) & i) == 0) {
+        waiting.flush(list, v, lane);
+        waiting.shared = common_threshold(list, sh_room, sh_share, wave, lane);
+      }
     }
   }
   if constexpr (TOP) waiting.flush(list, v, lane);
   st = stats_wave(st, c);
-  if constexpr (WAVES > 1) join_waves<A, WAVES, TOP>(st, list, c, wave, lane);
-  if (WAVES == 1 || a.splits == 1) {
+  const ChoiceArgs& z = late_args(a); // what follows reads its arguments anew: held over the steps they were spilled
+  if constexpr (WAVES > 1) {
+    __syncthreads();
+    join_waves<A, WAVES, TOP>(st, list, c, sh_room, sh_share, wave, lane);
+  }
+  if (WAVES == 1 || z.splits == 1) {
     if (WAVES == 1) {
-      finish_row<T>(a, row, b, r, st, lane, 64);
+      finish_row<T>(z, row, b, r, st, lane, 64);
     } else {
       __shared__ Stats<A> sh;
       if (threadIdx.x == 0) sh = st;
       __syncthreads();
-      finish_row<T>(a, row, b, r, sh, threadIdx.x, WAVES * 64);
+      finish_row<T>(z, row, b, r, sh, threadIdx.x, WAVES * 64);
     }
-    if (TOP && (WAVES == 1 || wave == 0)) finish_top(a, row, b, r, st, list, lane);
+    if (TOP && (WAVES == 1 || wave == 0)) finish_top(z, row, b, r, st, list, lane);
   } else if (wave == 0) {
-    char* at = static_cast<char*>(a.ws) + (row * a.splits + blockIdx.y) * (4 * (int64_t)sizeof(A) + (((int64_t)a.top * (sizeof(A) + 4) + 15) / 16 * 16));
+    char* at = static_cast<char*>(z.ws) + (row * z.splits + blockIdx.y) * (4 * (int64_t)sizeof(A) + (((int64_t)z.top * (sizeof(A) + 4) + 15) / 16 * 16));
     if (lane == 0) *reinterpret_cast<Partial<A>*>(at) = Partial<A>{st.m, st.s, st.t, (A)0};
-    if (TOP && lane < a.top) {
+    if (TOP && lane < z.top) {
       reinterpret_cast<A*>(at + 4 * sizeof(A))[lane] = list.key;
-      reinterpret_cast<uint32_t*>(at + 4 * sizeof(A) + a.top * sizeof(A))[lane] = list.idx;
+      reinterpret_cast<uint32_t*>(at + 4 * sizeof(A) + z.top * sizeof(A))[lane] = list.idx;
     }
   }
 }
@@ -338,7 +405,9 @@ __global__ __launch_bounds__(WAVES * 64) void choice_join_kernel(ChoiceArgs a) {
       list.consume_sorted(k, i, lane);
     }
   }
-  join_waves<A, WAVES, TOP>(st, list, c, wave, lane);
+  __shared__ WaveShare<A, WAVES> sh_share;
+  __shared__ WaitingRoom<A, 0> sh_room[TOP ? WAVES : 1];
+  join_waves<A, WAVES, TOP>(st, list, c, sh_room, sh_share, wave, lane);
   __shared__ Stats<A> sh;
   if (threadIdx.x == 0) sh = st;
   __syncthreads();
@@ -374,7 +443,7 @@ __global__ __launch_bounds__(256) void choice_grad_kernel(GradArgs a) {
   const int64_t unit = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = unit / a.stretches;
   if (row >= a.sc.rows) return;
-  const int64_t j0 = (unit - row * a.stretches) * (64 * E);
+  const int j0 = (int)(unit - row * a.stretches) * (64 * E);
   const int64_t b = (uint32_t)row / (uint32_t)a.sc.R, r = row - b * a.sc.R; // at most 2^25 rows
   const Row<T> v = row_view<T>(a.sc, b, r);
   A x[E];
@@ -429,7 +498,7 @@ __global__ __launch_bounds__(256) void choice_grad_kernel(GradArgs a) {
       const A g = (exp2_acc(w) * (base - gh * (ln2<A>() * not_below_low(w) + h)) + add[u * VEC + e]) * inv_T;
       from_acc(xe == neg_inf<A>() ? (A)0 : g, o.v[e]);
     }
-    const int64_t j = j0 + u * 64 * VEC + lane * VEC;
+    const int j = j0 + u * 64 * VEC + lane * VEC;
     if (j + VEC <= a.sc.M) {
       *reinterpret_cast<Pack<T, VEC>*>(out + j) = o;
     } else {
@@ -506,7 +575,7 @@ int pool_scores_view(gpx_ctx* ctx, const gpx_scores* x, PoolScores* out, const c
   if (!x) return no("null scores");
   if (x->dtype < GPX_DTYPE_F64 || x->dtype > GPX_DTYPE_F16) return no("dtype");
   if (x->pools < 0 || x->rows < 0 || x->candidates < 0) return no("negative size");
-  if (x->candidates > INT32_MAX - 65536) return no("more than 2^31 - 65536 candidates");
+  if (x->candidates > INT32_MAX - (1 << 20)) return no("more than 2^31 - 2^20 candidates");
   if (x->rows > 0 && x->pools > (int64_t)(1 << 25) / x->rows) return no("more than 2^25 rows");
   if (x->pools * x->rows > 0 && x->candidates > 0 && !x->d_scores) return no("null scores");
   if (!x->d_temperatures && !(x->temperature > 0 && x->temperature < INFINITY)) return no("the temperature must be positive and finite");

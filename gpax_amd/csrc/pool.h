@@ -115,10 +115,10 @@ __device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
     return __builtin_amdgcn_update_dpp(v, v, 0x128, 0xF, 0xF, false); // rotation of 16 by 8
   } else if constexpr (S == 16) { // first: odd rows replaced by the even ones below them; second: the other way round
     const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return (threadIdx.x & 16) ? r[0] : r[1];
+    return __builtin_amdgcn_inverse_ballot_w64(0xFFFF0000FFFF0000ull) ? r[0] : r[1];
   } else {
     const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return (threadIdx.x & 32) ? r[0] : r[1];
+    return __builtin_amdgcn_inverse_ballot_w64(0xFFFFFFFF00000000ull) ? r[0] : r[1];
   }
 }
 template <int S>
@@ -210,21 +210,21 @@ struct VecOf {
 
 // U vectors of VEC scores per lane: x[u * VEC + e] is candidate j0 + u * span + lane_j + e; -inf where there is none.
 // `span` (the team's lanes * VEC) and j0 are uniform over the team.  Addresses are clamped into the row instead of being
-// guarded one by one, so that every load of a step is in flight at once.
+// guarded one by one, so that every load of a step is in flight at once; they are a uniform base and a small offset per lane.
 template <typename T, int VEC, int U>
-__device__ __forceinline__ void load_step(const Row<T>& v, int64_t j0, int span, int lane_j, typename Acc<T>::type* x) {
+__device__ __forceinline__ void load_step(const Row<T>& v, int j0, int span, int lane_j, typename Acc<T>::type* x) {
   typedef typename Acc<T>::type A;
   const bool dense = v.xc == 1 && (!v.mask || v.mc == 1);
-  if (dense && j0 + (int64_t)U * span <= v.n) {
+  if (dense && j0 + U * span <= v.n) {
     Pack<T, VEC> p[U];
-    const T* at = v.x + j0 + lane_j;
+    const T* at = v.x + j0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) p[u] = *reinterpret_cast<const Pack<T, VEC>*>(at + u * span);
+    for (int u = 0; u < U; ++u) p[u] = *reinterpret_cast<const Pack<T, VEC>*>(at + (uint32_t)(u * span + lane_j));
     if (v.mask) {
       MaskPack<VEC> q[U];
-      const uint8_t* mat = v.mask + j0 + lane_j;
+      const uint8_t* mat = v.mask + j0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) q[u] = *reinterpret_cast<const MaskPack<VEC>*>(mat + u * span);
+      for (int u = 0; u < U; ++u) q[u] = *reinterpret_cast<const MaskPack<VEC>*>(mat + (uint32_t)(u * span + lane_j));
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -239,17 +239,21 @@ __device__ __forceinline__ void load_step(const Row<T>& v, int64_t j0, int span,
   }
   if (dense && v.n >= VEC) {
     // the end of the row: vectors that would cross it read the row's last VEC scores instead (and are dropped) ...
+    const int last = v.n - VEC, base = j0 < last ? j0 : last;
     Pack<T, VEC> p[U];
     MaskPack<VEC> q[U];
+    const T* at = v.x + base;
+    const uint8_t* mat = v.mask + base;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t j = j0 + (int64_t)u * span + lane_j, at = j + VEC <= v.n ? j : (int64_t)v.n - VEC;
-      p[u] = *reinterpret_cast<const Pack<T, VEC>*>(v.x + at);
-      if (v.mask) q[u] = *reinterpret_cast<const MaskPack<VEC>*>(v.mask + at);
+      const int j = j0 + u * span + lane_j;
+      const uint32_t off = (uint32_t)((j < last ? j : last) - base);
+      p[u] = *reinterpret_cast<const Pack<T, VEC>*>(at + off);
+      if (v.mask) q[u] = *reinterpret_cast<const MaskPack<VEC>*>(mat + off);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool in = j0 + (int64_t)u * span + lane_j + VEC <= v.n;
+      const bool in = j0 + u * span + lane_j <= last;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) x[u * VEC + e] = in && (!v.mask || q[u].v[e]) ? to_acc(p[u].v[e]) : neg_inf<A>();
     }
@@ -257,15 +261,14 @@ __device__ __forceinline__ void load_step(const Row<T>& v, int64_t j0, int span,
     if (v.n > j0 && (v.n - j0) % VEC != 0) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t base = j0 + (int64_t)u * span;
-        if (v.n < base || v.n >= base + span) continue; // uniform
+        const int first = j0 + u * span;
+        if (v.n < first || v.n >= first + span) continue; // uniform
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const int64_t j = base + lane_j + e;
-          const int64_t at = j < v.n ? j : (int64_t)v.n - 1;
-          const A a = to_acc(v.x[at]);
-          const bool there = !v.mask || v.mask[at] != 0;
-          if (base + lane_j + VEC > v.n && j < v.n) x[u * VEC + e] = there ? a : neg_inf<A>();
+          const int j = first + lane_j + e, off = j < v.n ? j : v.n - 1;
+          const A a = to_acc(v.x[off]);
+          const bool there = !v.mask || v.mask[off] != 0;
+          if (first + lane_j > last && j < v.n) x[u * VEC + e] = there ? a : neg_inf<A>();
         }
       }
     }
@@ -275,10 +278,10 @@ __device__ __forceinline__ void load_step(const Row<T>& v, int64_t j0, int span,
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const int64_t j = j0 + (int64_t)u * span + lane_j + e;
+      const int j = j0 + u * span + lane_j + e;
       A a = neg_inf<A>();
       if (v.n > 0) { // uniform
-        const int64_t at = j < v.n ? j : (int64_t)v.n - 1;
+        const int64_t at = j < v.n ? j : v.n - 1;
         a = to_acc(v.x[at * v.xc]);
         if (j >= v.n || (v.mask && !v.mask[at * v.mc])) a = neg_inf<A>();
       }

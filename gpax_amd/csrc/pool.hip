@@ -116,7 +116,7 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
     for (int e = 0; e < PER_LANE; ++e) acc[e] += sum[e * LANES + at];
   }
 #pragma unroll
-  for (int w = 0; w < U; ++w) store_sums<A, VEC>(a, b, blockIdx.x, (int64_t)w * LANES * VEC + at * VEC, acc + w * VEC);
+  for (int w = 0; w < U; ++w) store_sums<A, VEC>(a, b, blockIdx.x, w * LANES * VEC + at * VEC, acc + w * VEC);
 }
 
 // Second pass over longer pools: the rows' statistics are known, a workgroup sums 256 x VEC candidates over its share of rows.
@@ -1035,7 +1035,7 @@ int gpx_pool_evict(gpx_ctx* ctx, int dtype, int64_t pools, int64_t candidates, c
                    void* stream) {
   if (!ctx || ctx->device < 0) return -1;
   if (dtype != GPX_DTYPE_F64 && dtype != GPX_DTYPE_F32) return bad_arg(ctx, "gpx_pool_evict: weights are float64 or float32");
-  if (pools < 0 || candidates < 0 || pools > 65535 || candidates > INT32_MAX - 65536)
+  if (pools < 0 || candidates < 0 || pools > 65535 || candidates > INT32_MAX - (1 << 20))
     return bad_arg(ctx, "gpx_pool_evict: sizes");
   if (budget < 1 || budget > INT32_MAX) return bad_arg(ctx, "gpx_pool_evict: the budget must be positive");
   if (first < 0 || recent < 0 || first + recent > budget) return bad_arg(ctx, "gpx_pool_evict: first + recent exceed the budget");
