@@ -17,6 +17,7 @@ using namespace gpx;
 namespace {
 
 constexpr int TOP_MAX = 64;    // alternatives per row: one per lane of a wave
+constexpr int TWO_PER_LANE = 24; // lists longer than this: see Waiting::step (8 x 262144 float64 top 64: 26 -> 16 us)
 constexpr int INSERT_MAX = 10; // more than this many newcomers in one vector: sort and merge instead of inserting one by one
 
 struct ChoiceArgs {
@@ -37,11 +38,7 @@ __device__ __forceinline__ const ChoiceArgs& late_args(const ChoiceArgs&) {
   return *(const ChoiceArgs*)(const __attribute__((address_space(4))) ChoiceArgs*)p;
 }
 
-// A partial result in the workspace: statistics and the list, of one split of one row
-template <typename A>
-struct Partial {
-  A m, s, t, pad;
-};
+// A partial result in the workspace: Partial and the list, of one split of one row
 inline int64_t partial_bytes(int acc_size, int top) { return 4 * acc_size + round_up64((int64_t)top * (acc_size + 4), 16); }
 
 __device__ __forceinline__ float read_lane(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
@@ -168,7 +165,9 @@ struct WaitingRoom {
   A keys[64];
   uint32_t idx[64 * E + 64];
 };
-template <typename T, int VEC, int U>
+// TWO: for lists longer than TWO_PER_LANE, a better bound (where registers allow it: not for 16-bit scores, which need eight
+// waves a SIMD, nor for 64-bit ones in workgroups of 16 waves)
+template <typename T, int VEC, int U, bool TWO>
 struct Waiting {
   typedef typename Acc<T>::type A;
   WaitingRoom<A, U * VEC>& room; // this wave's
@@ -204,7 +203,22 @@ struct Waiting {
     if (many) {
       A sorted = cm;
       bitonic_values<2, 1>(sorted);
-      const A kth = read_lane(sorted, list.k - 1);
+      A kth = read_lane(sorted, list.k - 1);
+      if (TWO && list.k > TWO_PER_LANE) {
+        // for a long list the lanes' next best count too: of two sorted lists the larger of (a_i, b_63-i) are the best 64 of
+        // both; sorted again, the k-th of them.  (One score after the other: as a tree it takes twice the registers.)
+        A m2 = neg_inf<A>();
+#pragma unroll
+        for (int e = 0; e < U * VEC; ++e) {
+          m2 = fmax(m2, x[e] < cm ? x[e] : m2);
+          asm volatile("" : "+v"(m2));
+        }
+        bitonic_values<2, 1>(m2);
+        m2 = __shfl(m2, 63 - lane);
+        sorted = fmax(sorted, m2);
+        bitonic_values<64, 32>(sorted);
+        kth = read_lane(sorted, list.k - 1);
+      }
       bound = kth > bound ? kth : bound;
     }
 #pragma unroll
@@ -332,7 +346,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, sizeof(T) == 8 || WA
   const int first = WAVES == 1 ? 0 : ((int)blockIdx.y * WAVES + wave) * step;
   const int stride = WAVES == 1 ? step : a.splits * WAVES * step;
   const int steps = (int)(((uint32_t)v.n + (uint32_t)stride - 1) / (uint32_t)stride); // the same for all waves of the row's workgroup: they meet at barriers
-  Waiting<T, VEC, U> waiting{sh_room[TOP ? wave : 0], neg_inf<A>(), 0};
+  Waiting<T, VEC, U, (sizeof(T) == 4 || (sizeof(T) == 8 && WAVES != 16))> waiting{sh_room[TOP ? wave : 0], neg_inf<A>(), 0};
   for (int i = 0; i < steps; ++i) {
     const int j0 = first + i * stride;
     if (j0 < v.n) {
@@ -530,7 +544,7 @@ ChoicePlan choice_plan(int64_t rows, int64_t M) {
 }
 
 template <typename T, bool TOP>
-void choice_launch(const ChoiceArgs& a, ChoicePlan p, hipStream_t st) {
+void choice_launch(const ChoiceArgs& a, ChoicePlan p, hipStream_t st, bool join) {
   const unsigned rows = (unsigned)a.sc.rows;
   constexpr int U = StepOf<T>::wide, UN = StepOf<T>::narrow;
   if (p.waves == 1) {
@@ -542,22 +556,22 @@ void choice_launch(const ChoiceArgs& a, ChoicePlan p, hipStream_t st) {
     hipLaunchKernelGGL((choice_rows_kernel<T, 16, TOP, U>), dim3(rows), dim3(1024), 0, st, a);
   } else {
     hipLaunchKernelGGL((choice_rows_kernel<T, 4, TOP, U>), dim3(rows, p.splits), dim3(256), 0, st, a);
-    if (p.splits > 1) hipLaunchKernelGGL((choice_join_kernel<T, 16, TOP>), dim3(rows), dim3(1024), 0, st, a);
+    if (p.splits > 1 && join) hipLaunchKernelGGL((choice_join_kernel<T, 16, TOP>), dim3(rows), dim3(1024), 0, st, a);
   }
 }
 template <typename T>
-void choice_launch(const ChoiceArgs& a, ChoicePlan p, hipStream_t st) {
+void choice_launch(const ChoiceArgs& a, ChoicePlan p, hipStream_t st, bool join) {
   if (a.top > 0)
-    choice_launch<T, true>(a, p, st);
+    choice_launch<T, true>(a, p, st, join);
   else
-    choice_launch<T, false>(a, p, st);
+    choice_launch<T, false>(a, p, st, join);
 }
-void choice_launch(int dtype, const ChoiceArgs& a, ChoicePlan p, hipStream_t st) {
+void choice_launch(int dtype, const ChoiceArgs& a, ChoicePlan p, hipStream_t st, bool join = true) {
   switch (dtype) {
-    case GPX_DTYPE_F64: return choice_launch<double>(a, p, st);
-    case GPX_DTYPE_F32: return choice_launch<float>(a, p, st);
-    case GPX_DTYPE_BF16: return choice_launch<bf16_t>(a, p, st);
-    default: return choice_launch<f16_t>(a, p, st);
+    case GPX_DTYPE_F64: return choice_launch<double>(a, p, st, join);
+    case GPX_DTYPE_F32: return choice_launch<float>(a, p, st, join);
+    case GPX_DTYPE_BF16: return choice_launch<bf16_t>(a, p, st, join);
+    default: return choice_launch<f16_t>(a, p, st, join);
   }
 }
 int acc_size(int dtype) { return dtype == GPX_DTYPE_F64 ? 8 : 4; }
@@ -602,14 +616,15 @@ int pool_scores_view(gpx_ctx* ctx, const gpx_scores* x, PoolScores* out, const c
 }
 
 int64_t row_stats_workspace(int64_t rows, int64_t M, int dtype) { return choice_workspace(rows, M, dtype, 0); }
-int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, void* d_stats, void* d_ws, hipStream_t st) {
+int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, void* d_stats, void* d_parts, int* splits, hipStream_t st) {
   ChoiceArgs a{};
   const ChoicePlan p = choice_plan(sc.rows, sc.M);
   a.sc = sc;
   a.splits = p.splits;
   a.stats = d_stats;
-  a.ws = d_ws;
-  choice_launch(dtype, a, p, st);
+  a.ws = d_parts;
+  *splits = p.splits;
+  choice_launch(dtype, a, p, st, false);
   GPX_HIP(ctx, hipGetLastError());
   return 0;
 }

@@ -352,6 +352,30 @@ __device__ __forceinline__ A stats_entropy(const Stats<A>& a, A log2s) {
   return a.s == (A)0 ? (A)0 : ln2<A>() * (log2s - a.t / a.s);
 }
 
+// A partial result of one split of a row, as choice.hip leaves it (behind it, where there is one, the list of alternatives)
+template <typename A>
+struct Partial {
+  A m, s, t, pad;
+};
+// m and log2 s of a row from either form
+template <typename A>
+__device__ __forceinline__ void row_reference(const void* stats, const void* parts, int splits, int64_t row, A c, A& m, A& log2s) {
+  if (splits == 1) {
+    m = static_cast<const A*>(stats)[2 * row];
+    log2s = static_cast<const A*>(stats)[2 * row + 1];
+    return;
+  }
+  const Partial<A>* p = static_cast<const Partial<A>*>(parts) + row * splits;
+  m = neg_inf<A>();
+  for (int i = 0; i < splits; ++i) m = fmax(m, p[i].m);
+  A s = (A)0;
+  for (int i = 0; i < splits; ++i) { // (a split without candidates has s = 0, or NaN)
+    const A f = exp2_acc(not_below_low((p[i].m - m) * c));
+    s += p[i].m == neg_inf<A>() ? p[i].s : f * p[i].s;
+  }
+  log2s = log2_acc(s);
+}
+
 // pool.hip / choice.hip, host side
 int pool_scores_view(gpx_ctx* ctx, const gpx_scores* x, PoolScores* out, const char* what);
 struct DeviceGuard { // the caller's current device comes back whatever happens
@@ -371,8 +395,9 @@ struct DeviceGuard { // the caller's current device comes back whatever happens
   DeviceGuard(const DeviceGuard&) = delete;
   DeviceGuard& operator=(const DeviceGuard&) = delete;
 };
-// statistics of every row, [rows] x {m, log2 s}: pass one of pool_weights over pools too long for a workgroup (choice.hip)
-int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, void* d_stats, void* d_ws, hipStream_t st);
+// Statistics of every row, pass one of pool_weights over pools too long for a workgroup (choice.hip): rows x {m, log2 s} in
+// d_stats if *splits comes back as 1, else partial results of *splits parts of each row in d_parts
+int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, void* d_stats, void* d_parts, int* splits, hipStream_t st);
 int64_t row_stats_workspace(int64_t rows, int64_t M, int dtype);
 
 } // namespace gpx

@@ -19,7 +19,9 @@ struct WeightArgs {
   const void* weights;     // pools x M contiguous, or nullptr: zeros
   void* out;               // pools x M
   void* part;              // pools x groups x M partial sums when groups > 1
-  const void* stats;       // rows x {m, log2 s} (column pass)
+  const void* stats;       // column pass: rows x {m, log2 s}, or, where a row has several splits, ...
+  const void* parts;       // ... rows x splits partial results (choice.hip)
+  int splits;
   double decay;
   int groups;
 };
@@ -119,79 +121,92 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
   for (int w = 0; w < U; ++w) store_sums<A, VEC>(a, b, blockIdx.x, w * LANES * VEC + at * VEC, acc + w * VEC);
 }
 
-// Second pass over longer pools: the rows' statistics are known, a workgroup sums 256 x VEC candidates over its share of rows.
-// The next four rows are on their way while four are worked on; a mask that all rows share is read once.
+// Second pass over longer pools: a workgroup sums a tile of 256 x VEC x COL_VECS candidates over its share of rows.  What it
+// needs of a row (scale, reference, log of the sum, weight, length) it joins itself from the first pass's partial results, 64
+// rows at a time in LDS; the next row is on its way while one is worked on; a mask that all rows share is read once.  (64 x
+// 262144 float64: 36 us with one row of two vectors in flight, 37 with two rows or four vectors, 39 with one vector, 47 with
+// four rows of one vector.)
+template <typename A>
+struct ColumnRow {
+  A c, m, log2s, u;
+  int n;
+};
+constexpr int COL_VECS = 2, COL_BLOCK = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void pool_columns_kernel(WeightArgs a) {
   typedef typename Acc<T>::type A;
-  constexpr int VEC = VecOf<T>::value, ROWS = 4;
-  const int64_t b = blockIdx.z, M = a.sc.M;
-  const int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
+  constexpr int VEC = VecOf<T>::value, SPAN = 256 * VEC, U = COL_VECS, E = VEC * U;
+  __shared__ ColumnRow<A> rows[COL_BLOCK];
+  const int64_t b = blockIdx.z;
+  const int M = a.sc.M, j0 = (int)blockIdx.x * SPAN * U, mine = (int)threadIdx.x * VEC;
   const int64_t per = (a.sc.R + a.groups - 1) / a.groups;
   const int64_t r0 = per * blockIdx.y, r1 = r0 + per < a.sc.R ? r0 + per : a.sc.R;
-  A acc[VEC];
+  A acc[E];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) acc[e] = (A)0;
-  const bool whole = ((int64_t)blockIdx.x + 1) * 256 * VEC <= M && a.sc.xc == 1; // uniform: vectors, else score by score
+  for (int e = 0; e < E; ++e) acc[e] = (A)0;
+  auto place = [&](int e) { return j0 + (e / VEC) * SPAN + mine + e % VEC; };
+  const bool whole = j0 + SPAN * U <= M && a.sc.xc == 1; // uniform: vectors, else score by score
   const bool own_mask = a.sc.mask && a.sc.mr != 0;
   const T* x = static_cast<const T*>(a.sc.x) + b * a.sc.xb;
   const uint8_t* mask = a.sc.mask ? a.sc.mask + b * a.sc.mb : nullptr;
   uint32_t shared = ~0u; // which of this lane's candidates the mask of all rows allows
   if (mask && !own_mask)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (j + e >= M || !mask[(j + e) * a.sc.mc]) shared &= ~(1u << e);
-  auto load = [&](int64_t r, Pack<T, VEC>* p, uint32_t* ok) { // past the last row: the last one again, never used
+    for (int e = 0; e < E; ++e)
+      if (place(e) >= M || !mask[(int64_t)place(e) * a.sc.mc]) shared &= ~(1u << e);
+  Pack<T, VEC> next[U];
+  uint32_t next_ok = 0;
+  auto load = [&](int64_t r) {
+    const T* row = x + r * a.sc.xr;
+    next_ok = shared;
+    if (whole) {
+      const T* at = row + j0;
 #pragma unroll
-    for (int q = 0; q < ROWS; ++q) {
-      const int64_t rq = r + q < r1 ? r + q : r1 - 1;
-      const T* row = x + rq * a.sc.xr;
-      ok[q] = shared;
-      if (whole) {
-        p[q] = *reinterpret_cast<const Pack<T, VEC>*>(row + j);
-      } else {
+      for (int u = 0; u < U; ++u) next[u] = *reinterpret_cast<const Pack<T, VEC>*>(at + (uint32_t)(u * SPAN + mine));
+    } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) p[q].v[e] = row[(j + e < M ? j + e : M - 1) * a.sc.xc];
-      }
-      if (own_mask) {
-        const uint8_t* m = mask + rq * a.sc.mr;
+      for (int e = 0; e < E; ++e) next[e / VEC].v[e % VEC] = row[(place(e) < M ? place(e) : M - 1) * a.sc.xc];
+    }
+    if (own_mask) {
+      const uint8_t* m = mask + r * a.sc.mr;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (!m[(j + e < M ? j + e : M - 1) * a.sc.mc]) ok[q] &= ~(1u << e);
-      }
+      for (int e = 0; e < E; ++e)
+        if (!m[(place(e) < M ? place(e) : M - 1) * a.sc.mc]) next_ok &= ~(1u << e);
     }
   };
-  Pack<T, VEC> next[ROWS];
-  uint32_t next_ok[ROWS];
-  if (r0 < r1) load(r0, next, next_ok);
-  for (int64_t r = r0; r < r1; r += ROWS) {
-    Pack<T, VEC> p[ROWS];
-    uint32_t ok[ROWS];
-#pragma unroll
-    for (int q = 0; q < ROWS; ++q) {
-      p[q] = next[q];
-      ok[q] = next_ok[q];
+  if (r0 < r1) load(r0);
+  for (int64_t block = r0; block < r1; block += COL_BLOCK) {
+    __syncthreads();
+    if ((int)threadIdx.x < COL_BLOCK && block + threadIdx.x < r1) {
+      const int64_t r = block + threadIdx.x, row = b * a.sc.R + r;
+      ColumnRow<A> k;
+      k.c = temperature_scale(row_temperature<A>(a.sc, b, r));
+      k.u = a.row_weights ? static_cast<const A*>(a.row_weights)[row] : (A)1;
+      k.n = row_length(a.sc, b, r);
+      row_reference(a.stats, a.parts, a.splits, row, k.c, k.m, k.log2s);
+      rows[threadIdx.x] = k;
     }
-    if (r + ROWS < r1) load(r + ROWS, next, next_ok);
+    __syncthreads();
+    const int count = (int)(r1 - block < COL_BLOCK ? r1 - block : COL_BLOCK);
+    for (int q = 0; q < count; ++q) {
+      Pack<T, VEC> p[U];
 #pragma unroll
-    for (int q = 0; q < ROWS; ++q) {
-      if (r + q >= r1) break; // uniform, as all of the row's quantities
-      const int64_t row = b * a.sc.R + r + q;
-      const A u = a.row_weights ? static_cast<const A*>(a.row_weights)[row] : (A)1;
-      if (u == (A)0) continue;
-      const A c = temperature_scale(row_temperature<A>(a.sc, b, r + q));
-      const A m = static_cast<const A*>(a.stats)[2 * row], log2s = static_cast<const A*>(a.stats)[2 * row + 1];
-      const int n = row_length(a.sc, b, r + q);
+      for (int u = 0; u < U; ++u) p[u] = next[u];
+      const uint32_t ok = next_ok;
+      if (block + q + 1 < r1) load(block + q + 1);
+      const ColumnRow<A> k = rows[q];
+      if (k.u == (A)0) continue;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const A v = to_acc(p[q].v[e]);
-        const A w = u * exp2_acc((v - m) * c - log2s);
-        const bool in = j + e < n && ((ok[q] >> e) & 1) && v != neg_inf<A>();
+      for (int e = 0; e < E; ++e) {
+        const A v = to_acc(p[e / VEC].v[e % VEC]);
+        const A w = k.u * exp2_acc((v - k.m) * k.c - k.log2s);
+        const bool in = place(e) < k.n && ((ok >> e) & 1) && v != neg_inf<A>();
         acc[e] += in ? w : (A)0;
       }
     }
   }
-  store_sums<A, VEC>(a, b, blockIdx.y, j, acc);
+#pragma unroll
+  for (int u = 0; u < U; ++u) store_sums<A, VEC>(a, b, blockIdx.y, j0 + u * SPAN + mine, acc + u * VEC);
 }
 
 // decay w + the groups' partial sums in their order: 64 candidates per workgroup, the groups dealt to its four waves
@@ -904,7 +919,7 @@ WeightPlan weight_plan(int64_t pools, int64_t R, int64_t M, int dtype) {
   return WeightPlan{false, 4, 1};
 }
 int column_groups(int64_t pools, int64_t R, int64_t M, int vec) {
-  const int64_t tiles = (M + 256 * vec - 1) / (256 * vec) * (pools > 0 ? pools : 1);
+  const int64_t tile = 256 * vec * COL_VECS, tiles = (M + tile - 1) / tile * (pools > 0 ? pools : 1);
   int64_t g = (1024 + tiles - 1) / tiles; // workgroups that keep the memory busy
   const int64_t most = (R + 15) / 16;
   g = g > most ? most : g;
@@ -941,7 +956,8 @@ void weights_launch(const WeightArgs& a, const WeightPlan& p, int64_t pools, hip
     else
       hipLaunchKernelGGL((pool_weights_kernel<T, sizeof(T) == 8 ? 8 : 16, 1>), grid, dim3(p.waves * 64), 0, st, a);
   } else {
-    const unsigned tiles = (unsigned)((a.sc.M + 256 * VecOf<T>::value - 1) / (256 * VecOf<T>::value));
+    const int tile = 256 * VecOf<T>::value * COL_VECS;
+    const unsigned tiles = (unsigned)((a.sc.M + tile - 1) / tile);
     hipLaunchKernelGGL(pool_columns_kernel<T>, dim3(tiles, a.groups, (unsigned)pools), dim3(256), 0, st, a);
   }
   if (a.groups > 1) hipLaunchKernelGGL(pool_weights_join_kernel<A>, dim3((a.sc.M + 63) / 64, (unsigned)pools), dim3(256), 0, st, a);
@@ -1011,13 +1027,15 @@ int gpx_pool_weights(gpx_ctx* ctx, const gpx_scores* scores, const void* d_row_w
   a.out = d_out;
   a.part = d_workspace;
   a.stats = static_cast<char*>(d_workspace) + s.part;
+  a.parts = static_cast<char*>(d_workspace) + s.part + s.stats;
+  a.splits = 1;
   a.decay = decay;
   a.groups = p.one_pass ? p.groups : column_groups(scores->pools, a.sc.R, a.sc.M, vec_of(scores->dtype));
   DeviceGuard g(ctx->device);
   GPX_HIP(ctx, g.err);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (!p.one_pass && a.sc.rows > 0)
-    GPX_TRY(launch_row_stats(ctx, a.sc, scores->dtype, const_cast<void*>(a.stats), static_cast<char*>(d_workspace) + s.part + s.stats, st));
+    GPX_TRY(launch_row_stats(ctx, a.sc, scores->dtype, const_cast<void*>(a.stats), const_cast<void*>(a.parts), &a.splits, st));
   switch (scores->dtype) {
     case GPX_DTYPE_F64: weights_launch<double>(a, p, scores->pools, st); break;
     case GPX_DTYPE_F32: weights_launch<float>(a, p, scores->pools, st); break;
