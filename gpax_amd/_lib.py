@@ -936,6 +936,9 @@ _device_engines_lock = threading.Lock()
 def get_device_engine(device: int) -> Engine:
     """An engine on GPU `device` for operators on arrays that live there.  The default engine where it is that GPU's, else
     one kept beside it: the models' engine stays the default whatever device such a call is for."""
+    e = _device_engines.get(device)
+    if e is not None:
+        return e
     e = _default_engine
     if isinstance(e, Engine) and e.device == device:
         return e

@@ -10,6 +10,7 @@ import numpy as np
 from ..utils.utils import rng_from_key
 from .base_acq import ei, poi, ucb, ue
 from .penalties import compute_penalty
+from .pool import pool_evict, pool_weights
 
 
 def _compute_mean_and_var(rng_key, model, X, n: int, noiseless: bool, **kwargs) -> Tuple[np.ndarray, np.ndarray]:
@@ -70,6 +71,21 @@ def UE(rng_key, model, X, n: int = 1, noiseless: bool = False, penalty: Optional
     return _wrap(ue, rng_key, model, X, n, noiseless, penalty, recent_points, grid_indices, penalty_factor, kwargs)
 
 
+def _vi_draws(rng, model, X, n: int, noiseless: bool, **kwargs) -> np.ndarray:
+    """n joint draws (n, M) of a VI model at its point estimate, factored on the device: the exact models go through
+    ExactGP._predict (gpx_posterior + gpx_mvn_draw: chol(cov) and mean + L eps, gp.py:279-293); a model with its own posterior
+    (viSparseGP: Woodbury) hands its covariance to the device Cholesky (gpx_potrf)."""
+    from ..models.gp import ExactGP
+    params = model.get_samples()
+    if type(model).get_mvn_posterior is ExactGP.get_mvn_posterior:
+        _, draws = ExactGP._predict(model, rng, X, params, n, noiseless, **kwargs)
+        return draws
+    mean, cov = model.get_mvn_posterior(X, params, noiseless, **kwargs)
+    eps = rng.standard_normal((n, len(mean)))
+    L, info = model._engine().potrf(cov + 1e-12 * np.eye(len(mean)))
+    return np.stack([mean + L @ e for e in eps]) if info == 0 else np.full((n, len(mean)), np.nan)
+
+
 def Thompson(rng_key, model, X, n: int = 1, noiseless: bool = False, **kwargs) -> np.ndarray:
     """Thompson sampling (acquisition.py:488-524): one posterior sample of the GP parameters (HMC) or the
     point estimate (VI), then one function draw from its predictive distribution."""
@@ -84,16 +100,43 @@ def Thompson(rng_key, model, X, n: int = 1, noiseless: bool = False, **kwargs) -
         if n > 1:
             tsample = tsample.mean(1).squeeze()
         return tsample
-    # VI models: the reference only defines this branch for viDKL (sample_from_posterior); here the draw comes from
-    # the MVN posterior at the point estimate, factored on the device: the exact models go through
-    # ExactGP._predict (gpx_posterior + gpx_mvn_draw: chol(cov) and mean + L eps, gp.py:279-293); a model with its own
-    # posterior (viSparseGP: Woodbury) hands its covariance to the device Cholesky (gpx_potrf)
-    from ..models.gp import ExactGP
-    params = model.get_samples()
-    if type(model).get_mvn_posterior is ExactGP.get_mvn_posterior:
-        _, draws = ExactGP._predict(model, rng, X, params, 1, noiseless, **kwargs)
-        return draws
-    mean, cov = model.get_mvn_posterior(X, params, noiseless, **kwargs)
-    eps = rng.standard_normal(len(mean))
-    L, info = model._engine().potrf(cov + 1e-12 * np.eye(len(mean)))
-    return (mean + L @ eps)[None] if info == 0 else np.full((1, len(mean)), np.nan)
+    # VI models: the reference only defines this branch for viDKL (sample_from_posterior); here one draw from the MVN
+    # posterior at the point estimate
+    return _vi_draws(rng, model, X, 1, noiseless, **kwargs)
+
+
+def _gathered_weights(rng_key, model, X, temperature, maximize, n, noiseless, weights, decay, kwargs):
+    """(X as a column, weights gathered over the model's draws at X, number of draws that counted)"""
+    X = np.asarray(X, dtype=np.float64)
+    X = X[:, None] if X.ndim < 2 else X
+    if getattr(model, "mcmc", None) is not None:
+        _, y_sampled = model.predict(rng_key, X, n=n, noiseless=noiseless, **kwargs)
+        draws = np.asarray(y_sampled).reshape(-1, X.shape[0])
+    else:
+        draws = _vi_draws(rng_from_key(rng_key), model, X, n, noiseless, **kwargs)
+    counts = np.isfinite(draws).all(axis=1)  # a posterior sample whose factorisation failed has NaN draws: it has no say
+    w = pool_weights(draws if maximize else -draws, weights, decay=decay, row_weights=counts.astype(np.float64), temperature=temperature)
+    return X, w, int(counts.sum())
+
+
+def PBest(rng_key, model, X, temperature: float = 0.1, maximize: bool = False, n: int = 1, noiseless: bool = False,
+          **kwargs) -> np.ndarray:
+    """Probability of being the best candidate, as the softmax of every posterior draw over X at the given temperature (in
+    units of y; towards 0: the share of draws whose extremum each candidate is) gives it, averaged over the draws: n per
+    posterior sample (HMC) or n at the point estimate (VI).  What Thompson sampling (acquisition.py:488-524) picks from, one
+    draw at a time."""
+    _, w, count = _gathered_weights(rng_key, model, X, temperature, maximize, n, noiseless, None, 1.0, kwargs)
+    return w / count if count else np.full(len(w), np.nan)
+
+
+def shrink_pool(rng_key, model, X, budget: int, weights: Optional[np.ndarray] = None, decay: float = 1.0, first: int = 0,
+                recent: int = 0, temperature: float = 0.1, maximize: bool = False, n: int = 1, noiseless: bool = False,
+                **kwargs) -> Tuple[np.ndarray, np.ndarray, np.ndarray]:
+    """Cut a pool of candidates X (M, d) to at most `budget`: every candidate gathers, on top of `decay` times the weights it
+    has, its softmax probability over the model's draws (PBest), and those with the largest stay, the `first` first and
+    `recent` last in any case.  Returns (X, weights, indices) of what stayed, for the next step of the loop: the covariance
+    of the pool, M x M and factored per posterior sample, is what a step pays for."""
+    X, w, _ = _gathered_weights(rng_key, model, X, temperature, maximize, n, noiseless, weights, decay, kwargs)
+    e = pool_evict(w, budget, (X,), first=first, recent=recent)
+    k = int(e.lengths)
+    return e.payload[0][:k], e.weights[:k], e.indices[:k]

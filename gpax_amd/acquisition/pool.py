@@ -55,6 +55,8 @@ class PoolEviction(NamedTuple):
 
 
 def _is_torch(a) -> bool:
+    if _torch is not None:
+        return isinstance(a, _torch.Tensor)
     return type(a).__module__.partition(".")[0] == "torch"
 
 

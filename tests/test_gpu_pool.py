@@ -388,6 +388,53 @@ def test_other_streams_and_threads():
             assert torch.equal(u, v)
 
 
+def test_a_loop_of_the_operators_together():
+    """Draws come in, gather weights, the pool is cut, the rest of the draws' scores follow the kept indices, and the policy
+    over what is left names its choices: three rounds, every result against the plain implementations."""
+    rng = np.random.default_rng(11)
+    M, rows = 3000, 64
+    points = torch.as_tensor(rng.random((M, 2)), device="cuda")
+    w = torch.zeros(M, device="cuda", dtype=torch.float64)
+    hp, hw = host(points), host(w)
+    for budget in (2000, 700, 70):
+        x = torch.as_tensor(rng.standard_normal((rows, len(hw))), device="cuda")
+        w = acq.pool_weights(x, w, decay=0.9, temperature=0.4)
+        hw = ref.weights(host(x), hw, 0.9, T=0.4)
+        np.testing.assert_allclose(host(w), hw, rtol=1e-12)
+        e = acq.pool_evict(w, budget, (points,), first=3, recent=5)
+        i, n, hw, (hp,) = ref.evict(host(w), budget, [hp], 3, 5)  # of the device's own weights: equal ones are told apart by index
+        np.testing.assert_array_equal(host(e.indices), i)
+        assert int(e.lengths) == n == budget
+        np.testing.assert_array_equal(host(e.payload[0]), hp)
+        w, points = e.weights, e.payload[0]
+        kept = x[:, e.indices]
+        r = acq.choice_logprobs(kept, e.indices.new_zeros(rows, 1), temperature=0.4, top=5)
+        check_choice(r, kept, "float64", e.indices.new_zeros(rows, 1), 0.4, None, None, 5)
+        g = acq.choice_logprobs_grad(kept, r, e.indices.new_zeros(rows, 1), grad_logprobs=torch.ones_like(r.logprobs), temperature=0.4)
+        assert float(g.sum(1).abs().max()) < 1e-12  # a softmax's gradient sums to nothing
+
+
+def test_models_feed_the_pool_on_the_gpu():
+    import bench_inputs
+    from gpax_amd import ExactGP
+    from gpax_amd.utils import get_keys
+    _lib.set_engine(None)
+    X, y, Xn, _ = bench_inputs.synthetic_problem(60, 2, 200, seed=3)
+    m = ExactGP(2, "Matern")
+    m.fit(get_keys()[0], X, y, num_warmup=20, num_samples=20, progress_bar=False, print_summary=False)
+    _, draws = m.predict(get_keys()[1], Xn, n=3)
+    want = ref.weights(-np.asarray(draws).reshape(-1, 200), T=0.3) / 60
+    p = acq.PBest(get_keys()[1], m, Xn, temperature=0.3, n=3)
+    np.testing.assert_allclose(p, want, rtol=1e-11)
+    Xk, w, idx = acq.shrink_pool(get_keys()[1], m, Xn, 50, recent=4, temperature=0.3, n=3)
+    keep = np.sort(np.concatenate([np.argsort(-want[:196], kind="stable")[:46], np.arange(196, 200)]))
+    np.testing.assert_array_equal(idx, keep)
+    np.testing.assert_array_equal(Xk, Xn[keep])
+    np.testing.assert_allclose(w, 60 * want[keep], rtol=1e-11)
+    r = acq.choice_logprobs(acq.UCB(get_keys()[1], m, Xk, n=2), top=4, temperature=0.1)
+    assert r.top_indices.shape == (4,) and np.all(np.diff(r.top_logprobs) <= 0) and np.exp(r.top_logprobs).sum() <= 1
+
+
 def test_refusals_of_tensors():
     x = torch.zeros(3, 10, device="cuda")
     bad = [lambda: acq.choice_logprobs(x.cpu()), lambda: acq.choice_logprobs(x.int()), lambda: acq.choice_logprobs(x.requires_grad_(True)),

@@ -100,6 +100,46 @@ def test_eviction_moves_points_and_reports_lengths():
     assert one.indices.tolist() == [1, 3] and one.lengths.shape == () and one.payload[1].tolist() == [1, 3]
 
 
+def test_models_feed_the_pool():
+    """PBest and shrink_pool on a fitted HMC and a VI model: the draws of predict through the plain implementations."""
+    import bench_inputs
+    from gpax_amd.models import ExactGP, viGP
+    from gpax_amd.utils import get_keys
+    Xt, y, Xn, _ = bench_inputs.synthetic_problem(20, 1, 15, seed=2)
+    m = ExactGP(1, "RBF")
+    m.fit(get_keys()[0], Xt, y, num_warmup=15, num_samples=15, progress_bar=False, print_summary=False)
+    _, draws = m.predict(get_keys()[1], Xn, n=2)
+    want = ref.weights(-draws.reshape(-1, 15), T=0.2) / 30
+    p = acq.PBest(get_keys()[1], m, Xn, temperature=0.2, n=2)
+    np.testing.assert_allclose(p, want, rtol=1e-12)
+    assert abs(p.sum() - 1) < 1e-12
+    Xk, w, idx = acq.shrink_pool(get_keys()[1], m, Xn[:, 0], 6, weights=np.full(15, 4.0), decay=0.5, recent=1, temperature=0.2, n=2)
+    full = 2.0 + 30 * want
+    keep = np.sort(np.append(np.argsort(-full[:14], kind="stable")[:5], 14))
+    assert idx.tolist() == keep.tolist() and Xk.shape == (6, 1)
+    np.testing.assert_allclose(w, full[keep], rtol=1e-12)
+    np.testing.assert_array_equal(Xk, Xn[keep])
+    v = viGP(1, "Matern")
+    v.fit(get_keys()[0], Xt, y, num_steps=10, progress_bar=False, print_summary=False)
+    q = acq.PBest(get_keys()[1], v, Xn, n=7, maximize=True)
+    assert q.shape == (15,) and abs(q.sum() - 1) < 1e-12
+    assert acq.shrink_pool(get_keys()[1], v, Xn, 40)[2].tolist() == list(range(15))
+
+
+def test_draws_that_failed_have_no_say(monkeypatch):
+    class Model:
+        mcmc = object()
+
+        def predict(self, key, X, n=1, noiseless=False, **kw):
+            d = np.random.default_rng(0).standard_normal((4, n, len(X)))
+            d[2] = np.nan
+            return d.mean((0, 1)), d
+
+    p = acq.PBest(0, Model(), np.zeros((5, 1)), n=3)
+    d = np.delete(Model().predict(0, np.zeros((5, 1)), n=3)[1], 2, axis=0).reshape(-1, 5)
+    np.testing.assert_allclose(p, ref.weights(-d, T=0.1) / 9, rtol=1e-12)
+
+
 X = np.zeros((3, 10))
 BAD = {
     "four dimensions": lambda: acq.choice_logprobs(X[None, None]), "a scalar": lambda: acq.choice_logprobs(np.float64(1)),
