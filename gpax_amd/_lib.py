@@ -940,7 +940,7 @@ def get_device_engine(device: int) -> Engine:
     if e is not None:
         return e
     e = _default_engine
-    if isinstance(e, Engine) and e.device == device:
+    if isinstance(e, Engine) and e.device == device and e._ctx:
         return e
     with _device_engines_lock:
         e = _device_engines.get(device)

@@ -102,7 +102,10 @@ class _Device:
         if _torch is None:
             _bind_torch()
         self.ref, self.index = ref, ref.get_device()
-        self.engine = _lib.get_device_engine(self.index)
+        self.engine = _lib._device_engines.get(self.index)
+        if self.engine is None:  # (making one sets the current device)
+            with _torch.cuda.device(self.index):
+                self.engine = _lib.get_device_engine(self.index)
 
     def take(self, a, name: str, kinds: Sequence[str], contiguous: bool = False):
         if not isinstance(a, _torch.Tensor) or a.get_device() != self.index:  # -1: on the host
@@ -163,6 +166,8 @@ class _Host:
             if want == "bool" or a.dtype.kind not in "iuf" or (want == "int64" and a.dtype.kind == "f"):
                 raise ValueError(f"{name} has dtype {a.dtype.name}; expected {' or '.join(kinds)}")
             a = a.astype(want)
+        elif not a.dtype.isnative:
+            a = a.astype(a.dtype.newbyteorder("="))
         return np.ascontiguousarray(a) if a.ndim else a.copy()
 
     def kind(self, a) -> str:
@@ -415,7 +420,7 @@ def pool_weights(scores, weights=None, *, decay: float = 1.0, row_weights=None, 
     Args:
         scores: (M,), (rows, M) or (pools, rows, M)
         weights: weights gathered before, (M,) or (pools, M), of the accumulator's type; None: zeros
-        decay: factor on them, finite and not negative
+        decay: factor on them, finite and not negative; 0 forgets them, whatever they are
         row_weights: factor of each row, of the accumulator's type, shape scores.shape[:-1]; a row of weight 0 is not read
         temperature, mask, lengths: as for choice_logprobs
         out: array for the result (may be `weights`)
@@ -433,7 +438,7 @@ def pool_weights(scores, weights=None, *, decay: float = 1.0, row_weights=None, 
         raise ValueError("more than 65535 pools")
     shape = (pol.pools, pol.M) if len(pol.shape) == 3 else (pol.M,)
     w = u = None
-    if weights is not None:
+    if weights is not None and decay != 0.0:
         w = sp.take(weights, "weights", (pol.acc,), contiguous=True)
         if tuple(w.shape) != shape:
             raise ValueError(f"weights have shape {tuple(w.shape)}; expected {shape}")

@@ -882,23 +882,26 @@ __global__ __launch_bounds__(1024) void pool_evict_put_kernel(EvictArgs a) {
   if (c == 0 && tid == 0) a.new_lengths[b] = cut.keep;
 }
 
-// Payload rows too long for that: `row` bytes each, moved in units; zeros where nothing stayed.
+// Payload rows too long for that, of one pool a grid row: 2^log_lanes lanes a row, moved in units; zeros where nothing stayed.
 template <typename Unit>
-__global__ __launch_bounds__(256) void pool_gather_kernel(const int64_t* indices, const Unit* src, Unit* dst, int64_t total, int64_t K, int64_t M, int units) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / units, u = i - row * units, b = row / K;
-    const int64_t j = indices[row];
-    Unit v{};
-    if (j >= 0) v = src[(b * M + j) * units + u];
-    dst[i] = v;
+__global__ __launch_bounds__(256) void pool_gather_kernel(const int64_t* indices, const Unit* src, Unit* dst, int64_t K, int64_t M, int units, int log_lanes) {
+  const int64_t b = blockIdx.y;
+  const int lanes = 1 << log_lanes, at = threadIdx.x & (lanes - 1), per = 256 >> log_lanes;
+  for (int64_t p = (int64_t)blockIdx.x * per + (threadIdx.x >> log_lanes); p < K; p += (int64_t)gridDim.x * per) {
+    const int64_t j = indices[b * K + p];
+    const Unit* s = src + (b * M + (j < 0 ? 0 : j)) * units;
+    Unit* d = dst + (b * K + p) * units;
+    for (int u = at; u < units; u += lanes) d[u] = j < 0 ? Unit{} : s[u];
   }
 }
 template <typename Unit>
 void gather_launch(const int64_t* indices, const void* src, void* dst, int64_t pools, int64_t K, int64_t M, int64_t row_bytes, hipStream_t st) {
-  const int64_t units = row_bytes / (int64_t)sizeof(Unit), total = pools * K * units;
-  const int64_t blocks = (total + 255) / 256;
-  hipLaunchKernelGGL(pool_gather_kernel<Unit>, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st, indices,
-                     static_cast<const Unit*>(src), static_cast<Unit*>(dst), total, K, M, (int)units);
+  const int64_t units = row_bytes / (int64_t)sizeof(Unit);
+  int log_lanes = 0;
+  while (log_lanes < 8 && ((int64_t)1 << log_lanes) < units) ++log_lanes;
+  const int64_t per = 256 >> log_lanes, blocks = (K + per - 1) / per;
+  hipLaunchKernelGGL(pool_gather_kernel<Unit>, dim3((unsigned)(blocks < 65536 ? blocks : 65536), (unsigned)pools), dim3(256), 0, st, indices,
+                     static_cast<const Unit*>(src), static_cast<Unit*>(dst), K, M, (int)units, log_lanes);
 }
 
 // Teams that work off a pool's rows in the one-pass kernel, and groups (workgroups) of them.
@@ -1023,7 +1026,7 @@ int gpx_pool_weights(gpx_ctx* ctx, const gpx_scores* scores, const void* d_row_w
   if (s.total > 0 && (!d_workspace || workspace_bytes < s.total))
     return bad_arg(ctx, "gpx_pool_weights: workspace too small (gpx_pool_weights_workspace)");
   a.row_weights = d_row_weights;
-  a.weights = d_weights;
+  a.weights = decay == 0.0 ? nullptr : d_weights;
   a.out = d_out;
   a.part = d_workspace;
   a.stats = static_cast<char*>(d_workspace) + s.part;

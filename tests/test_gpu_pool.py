@@ -229,6 +229,8 @@ def test_pool_weights(kind, shape):
         close(host(got), want, tol, "weights")
         assert torch.equal(got, acq.pool_weights(x, w, decay=0.75, row_weights=u, temperature=T, mask=mask, lengths=lengths))
         if old:
+            nothing = acq.pool_weights(x, torch.full_like(w, math.nan), decay=0.0, row_weights=u, temperature=T, mask=mask, lengths=lengths)
+            assert torch.equal(nothing, acq.pool_weights(x, row_weights=u, temperature=T, mask=mask, lengths=lengths))
             acq.pool_weights(x, w, decay=0.75, row_weights=u, temperature=T, mask=mask, lengths=lengths, out=w)
             assert torch.equal(w, got)
 
@@ -256,6 +258,8 @@ def test_pool_evict(kind, shape, budget):
     put = lambda a, k=kind: torch.as_tensor(a, device="cuda").to(getattr(torch, k))
     plain = rng.lognormal(0, 3, shape)
     values = {"plain": plain, "zeros": np.where(rng.random(shape) < 0.9, 0.0, plain), "same": np.full(shape, 0.3), "few": rng.integers(0, 3, shape) - 1.0,
+              # all but one agree in the 24 highest bits in which they differ from it
+              "outlier": np.where(np.arange(M) == M // 2, 1e30, 1.0 + rng.integers(0, 50, shape) * 2.0 ** (-23 if kind == "float32" else -52)),
               "close": 1.0 + rng.integers(0, 50, shape) * 2.0 ** (-23 if kind == "float32" else -52), "signs": rng.standard_normal(shape),
               "special": np.where(rng.random(shape) < 0.2, rng.choice([np.nan, np.inf, -np.inf, -0.0, 0.0], shape), plain)}
     lens = torch.as_tensor(rng.integers(-1, M + 2, shape[:-1]), device="cuda")
@@ -272,8 +276,9 @@ def test_evict_moves_payload_of_every_width():
     w = torch.as_tensor(rng.random((3, 500)), device="cuda")
     payload = [torch.as_tensor(rng.integers(0, 255, (3, 500) + s), device="cuda").to(t) for s, t in
                [((), torch.uint8), ((3,), torch.uint8), ((5,), torch.int16), ((3,), torch.int32), ((3,), torch.int64), ((2,), torch.float64),
-                ((0,), torch.float32), ((4, 64), torch.float32)]]
+                ((0,), torch.float32), ((4, 64), torch.float32), ((71,), torch.uint8), ((45,), torch.int16), ((19,), torch.int32), ((601,), torch.float64)]]
     check_evict(w, 77, payload, first=3)
+    check_evict(w, 77, payload, first=3, lengths=torch.tensor([0, 30, 400], device="cuda"))
     view = torch.as_tensor(rng.random((3, 500, 5)), device="cuda")[:, :, 1:4]
     check_evict(w, 77, (view,), recent=9)
 

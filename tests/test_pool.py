@@ -83,6 +83,13 @@ def test_staging_of_every_argument(shape, kind):
                 assert w.shape == (shape[:1] + (M,) if len(shape) == 3 else (M,))
 
 
+def test_arrays_of_the_other_byte_order():
+    x = np.random.default_rng(3).standard_normal((2, 6))
+    a, b = acq.choice_logprobs(x.astype(">f8"), np.zeros((2, 1), ">i8"), top=2), acq.choice_logprobs(x, np.zeros((2, 1), int), top=2)
+    np.testing.assert_array_equal(a.logprobs, b.logprobs)
+    np.testing.assert_array_equal(acq.pool_evict(x.astype(">f8"), 3).weights, acq.pool_evict(x, 3).weights)
+
+
 def test_one_choice_a_row_and_lists():
     r = acq.choice_logprobs([[0, 1], [2, 3]], [1, 0])
     np.testing.assert_allclose(r.logprobs, [-math.log(1 + math.exp(-1)), -1 - math.log(1 + math.exp(-1))])
