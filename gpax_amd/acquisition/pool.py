@@ -269,11 +269,12 @@ class _Policy:
             ts = _pad2(_broadcast_strides(tuple(t.shape), space.strides(t), lead, "temperature"))
             if space.host and not (np.all(t > 0) and np.all(np.isfinite(t))):
                 raise ValueError("the temperature must be positive and finite")
-        self._rest = (p, r, M, *_pad3(space.strides(x))), ms, ls, (*ts, T, _DTYPES[kind], n64)
+        self._fields = (p, r, M, *_pad3(space.strides(x))), ms, ls, (*ts, T, _DTYPES[kind], n64)
 
     def struct(self, ptr) -> bytes:
-        a, ms, ls, rest = self._rest
-        return _pack(ptr(self.scores), *a, ptr(self.mask), *ms, ptr(self.lengths), *ls, ptr(self.temps), *rest)
+        a, ms, ls, rest = self._fields
+        return _pack(ptr(self.scores), *a, ptr(self.mask) if self.mask is not None else 0, *ms,
+                     ptr(self.lengths) if self.lengths is not None else 0, *ls, ptr(self.temps) if self.temps is not None else 0, *rest)
 
     def inputs(self):
         return self.scores, self.mask, self.lengths, self.temps
@@ -502,19 +503,20 @@ def pool_evict(weights, budget: int, payload: Sequence = (), *, first: int = 0, 
     if len(payload) > MAX_PAYLOAD:
         raise ValueError(f"{len(payload)} payload arrays; at most {MAX_PAYLOAD}")
     moved, moved_out, row_bytes = [], [], []
-    for i, a in enumerate(payload):
-        kinds = _PAYLOAD if not sp.host else (np.asarray(a).dtype.name,)
-        a = sp.take(a, f"payload[{i}]", kinds, contiguous=True)
+    dims = len(lead) + 1
+    for a in payload:
+        a = sp.take(a, "payload", _PAYLOAD if not sp.host else (np.asarray(a).dtype.name,), contiguous=True)
+        shape = tuple(a.shape)
         if sp.host and a.dtype.kind not in "biufc":
-            raise ValueError(f"payload[{i}] has dtype {a.dtype.name}; expected numbers")
-        if tuple(a.shape[: len(lead) + 1]) != lead + (M,):
-            raise ValueError(f"payload[{i}] has shape {tuple(a.shape)}; expected {lead + (M,)} + (...)")
+            raise ValueError(f"payload has dtype {a.dtype.name}; expected numbers")
+        if shape[:dims] != lead + (M,):
+            raise ValueError(f"payload has shape {shape}; expected {lead + (M,)} + (...)")
+        row = shape[dims:]
         moved.append(a)
-        moved_out.append(sp.new(lead + (budget,) + tuple(a.shape[len(lead) + 1:]), sp.kind(a)))
-        size = a.itemsize if sp.host else a.element_size()
-        row_bytes.append(math.prod(a.shape[len(lead) + 1:]) * size)
+        moved_out.append(sp.new(lead + (budget,) + row, sp.kind(a)))
+        row_bytes.append(math.prod(row) * (a.itemsize if sp.host else a.element_size()))
         if row_bytes[-1] > (1 << 31) - 1:
-            raise ValueError(f"payload[{i}] has rows of 2 GiB or more")
+            raise ValueError("payload has rows of 2 GiB or more")
     indices, left, w_out = sp.new(lead + (budget,), "int64"), sp.new(lead, "int64"), sp.new(lead + (budget,), sp.kind(w))
 
     dtype = _DTYPES[sp.kind(w)]

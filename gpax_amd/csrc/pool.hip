@@ -31,12 +31,13 @@ constexpr int TEAMS = 8;     // rows at a time of a workgroup whose teams are si
 // the largest team: 16 sums and 16 scores of 64 bits do not fit the 128 registers that 16 waves leave each lane
 inline int team_waves(int dtype) { return dtype == GPX_DTYPE_F64 ? 8 : 16; }
 
-// a finished sum of candidates j .. j + VEC: straight to the output, or to this group's partial sums
+// finished sums of candidates j .. j + VEC, of them those from `from` on: straight to the output, or to this group's partial sums
 template <typename A, int VEC>
-__device__ __forceinline__ void store_sums(const WeightArgs& a, int64_t b, int group, int64_t j, const A* acc) {
+__device__ __forceinline__ void store_sums(const WeightArgs& a, int64_t b, int group, int64_t from, int64_t j, const A* acc) {
   const int64_t M = a.sc.M;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
+    if (j + e < from) continue;
     if (j + e >= M) return;
     if (a.groups > 1) {
       static_cast<A*>(a.part)[(b * a.groups + group) * M + j + e] = acc[e];
@@ -67,6 +68,7 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
     const Row<T> v = row_view<T>(a.sc, b, r);
     A x[PER_LANE];
     load_step<T, VEC, U>(v, 0, LANES * VEC, at * VEC, x);
+    const int live = (v.n + LANES * VEC - 1) / (LANES * VEC); // vectors of the lanes that the row reaches into
     A m = x[0];
 #pragma unroll
     for (int e = 1; e < PER_LANE; ++e) m = fmax(m, x[e]);
@@ -80,9 +82,13 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
     const A ref = finite_max(m);
     A s = (A)0;
 #pragma unroll
-    for (int e = 0; e < PER_LANE; ++e) {
-      x[e] = exp2_acc((x[e] - ref) * c);
-      s += x[e];
+    for (int w = 0; w < U; ++w) {
+      if (w >= live) break; // uniform
+#pragma unroll
+      for (int e = w * VEC; e < (w + 1) * VEC; ++e) {
+        x[e] = exp2_acc((x[e] - ref) * c);
+        s += x[e];
+      }
     }
     s = wave_sum(s);
     if (WAVES > 1) {
@@ -101,7 +107,11 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
       for (int e = 0; e < PER_LANE; ++e) acc[e] += x[e] == neg_inf<A>() ? (A)0 : f;
     } else {
 #pragma unroll
-      for (int e = 0; e < PER_LANE; ++e) acc[e] = fma(x[e], f, acc[e]);
+      for (int w = 0; w < U; ++w) {
+        if (w >= live) break;
+#pragma unroll
+        for (int e = w * VEC; e < (w + 1) * VEC; ++e) acc[e] = fma(x[e], f, acc[e]);
+      }
     }
   }
   if (NTEAMS > 1) { // the teams' sums in the order of the teams, into the first one's registers
@@ -118,95 +128,112 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
     for (int e = 0; e < PER_LANE; ++e) acc[e] += sum[e * LANES + at];
   }
 #pragma unroll
-  for (int w = 0; w < U; ++w) store_sums<A, VEC>(a, b, blockIdx.x, w * LANES * VEC + at * VEC, acc + w * VEC);
+  for (int w = 0; w < U; ++w) store_sums<A, VEC>(a, b, blockIdx.x, 0, w * LANES * VEC + at * VEC, acc + w * VEC);
 }
 
-// Second pass over longer pools: a workgroup sums a tile of 256 x VEC x COL_VECS candidates over its share of rows.  What it
-// needs of a row (scale, reference, log of the sum, weight, length) it joins itself from the first pass's partial results, 64
-// rows at a time in LDS; the next row is on its way while one is worked on; a mask that all rows share is read once.  (64 x
-// 262144 float64: 36 us with one row of two vectors in flight, 37 with two rows or four vectors, 39 with one vector, 47 with
-// four rows of one vector.)
+// Second pass over longer pools: a workgroup sums a tile of 256 lanes' vectors over its share of rows.  What it needs of a row
+// (scale, reference, log of the sum, weight, length) it joins itself from the first pass's partial results, 64 rows at a time in
+// LDS; the next row that reaches into the tile is on its way while one is worked on; a mask that all rows share is read once.
+// A vector that would cross the end of the pool starts earlier, and only its own candidates are written.  DENSE: candidates (and
+// mask bytes) side by side.
+constexpr int COL_BLOCK = 64;
+constexpr int col_vecs(int size) { return size == 2 ? 1 : 2; } // vectors a lane holds of a row (one is 8 scores of 16 bits)
 template <typename A>
 struct ColumnRow {
   A c, m, log2s, u;
   int n;
 };
-constexpr int COL_VECS = 2, COL_BLOCK = 64;
-template <typename T>
+template <typename T, bool DENSE>
 __global__ __launch_bounds__(256) void pool_columns_kernel(WeightArgs a) {
   typedef typename Acc<T>::type A;
-  constexpr int VEC = VecOf<T>::value, SPAN = 256 * VEC, U = COL_VECS, E = VEC * U;
+  constexpr int VEC = VecOf<T>::value, SPAN = 256 * VEC, U = col_vecs(sizeof(T)), E = VEC * U;
   __shared__ ColumnRow<A> rows[COL_BLOCK];
   const int64_t b = blockIdx.z;
-  const int M = a.sc.M, j0 = (int)blockIdx.x * SPAN * U, mine = (int)threadIdx.x * VEC;
+  const int M = a.sc.M, j0 = (int)blockIdx.x * SPAN * U;
   const int64_t per = (a.sc.R + a.groups - 1) / a.groups;
   const int64_t r0 = per * blockIdx.y, r1 = r0 + per < a.sc.R ? r0 + per : a.sc.R;
   A acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = (A)0;
-  auto place = [&](int e) { return j0 + (e / VEC) * SPAN + mine + e % VEC; };
-  const bool whole = j0 + SPAN * U <= M && a.sc.xc == 1; // uniform: vectors, else score by score
-  const bool own_mask = a.sc.mask && a.sc.mr != 0;
+  int off[U]; // this lane's vectors; a pool that comes here has more than a vector's candidates
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int start = j0 + u * SPAN + (int)threadIdx.x * VEC;
+    off[u] = start < M - VEC ? start : M - VEC;
+  }
   const T* x = static_cast<const T*>(a.sc.x) + b * a.sc.xb;
   const uint8_t* mask = a.sc.mask ? a.sc.mask + b * a.sc.mb : nullptr;
-  uint32_t shared = ~0u; // which of this lane's candidates the mask of all rows allows
-  if (mask && !own_mask)
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (place(e) >= M || !mask[(int64_t)place(e) * a.sc.mc]) shared &= ~(1u << e);
   Pack<T, VEC> next[U];
-  uint32_t next_ok = 0;
-  auto load = [&](int64_t r) {
-    const T* row = x + r * a.sc.xr;
-    next_ok = shared;
-    if (whole) {
-      const T* at = row + j0;
+  MaskPack<VEC> next_mask[U];
+  auto load_mask = [&](const uint8_t* m) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) next[u] = *reinterpret_cast<const Pack<T, VEC>*>(at + (uint32_t)(u * SPAN + mine));
-    } else {
+    for (int u = 0; u < U; ++u) {
+      if (DENSE) {
+        next_mask[u] = *reinterpret_cast<const MaskPack<VEC>*>(m + (uint32_t)off[u]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) next[e / VEC].v[e % VEC] = row[(place(e) < M ? place(e) : M - 1) * a.sc.xc];
-    }
-    if (own_mask) {
-      const uint8_t* m = mask + r * a.sc.mr;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (!m[(place(e) < M ? place(e) : M - 1) * a.sc.mc]) next_ok &= ~(1u << e);
+        for (int e = 0; e < VEC; ++e) next_mask[u].v[e] = m[(off[u] + e) * a.sc.mc];
+      }
     }
   };
-  if (r0 < r1) load(r0);
+  auto load = [&](int64_t r) {
+    const T* row = x + r * a.sc.xr;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (DENSE) {
+        next[u] = *reinterpret_cast<const Pack<T, VEC>*>(row + (uint32_t)off[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) next[u].v[e] = row[(off[u] + e) * a.sc.xc];
+      }
+    }
+    if (mask && a.sc.mr != 0) load_mask(mask + r * a.sc.mr);
+  };
+  if (mask && a.sc.mr == 0) load_mask(mask);
+#pragma unroll 1
   for (int64_t block = r0; block < r1; block += COL_BLOCK) {
     __syncthreads();
-    if ((int)threadIdx.x < COL_BLOCK && block + threadIdx.x < r1) {
-      const int64_t r = block + threadIdx.x, row = b * a.sc.R + r;
+    // 16 lanes a row, a partial result each
+    const int count = (int)(r1 - block < COL_BLOCK ? r1 - block : COL_BLOCK);
+#pragma unroll 1
+    for (int i = 0; i * 16 < count; ++i) {
+      const int local = i * 16 + ((int)threadIdx.x >> 4);
+      const int64_t r = block + local < r1 ? block + local : r1 - 1, row = b * a.sc.R + r;
       ColumnRow<A> k;
       k.c = temperature_scale(row_temperature<A>(a.sc, b, r));
       k.u = a.row_weights ? static_cast<const A*>(a.row_weights)[row] : (A)1;
       k.n = row_length(a.sc, b, r);
-      row_reference(a.stats, a.parts, a.splits, row, k.c, k.m, k.log2s);
-      rows[threadIdx.x] = k;
+      row_reference(a.stats, a.parts, a.splits, row, k.c, (int)threadIdx.x & 15, k.m, k.log2s);
+      if (k.u == (A)0 || k.m == neg_inf<A>()) k.n = 0; // weight 0, or nothing that may be chosen (and no NaN: that has no largest)
+      if (k.u != (A)0 && k.log2s != k.log2s) k.n = row_length(a.sc, b, r);
+      if ((threadIdx.x & 15) == 0) rows[local] = k;
     }
     __syncthreads();
-    const int count = (int)(r1 - block < COL_BLOCK ? r1 - block : COL_BLOCK);
-    for (int q = 0; q < count; ++q) {
+    ColumnRow<A> k = rows[0], kn = k;
+    if (j0 < k.n) load(block); // uniform: the row reaches into the tile
+#pragma unroll 1
+    for (int q = 0; q < count; ++q, k = kn) {
+      kn = rows[q + 1 < count ? q + 1 : q];
       Pack<T, VEC> p[U];
+      MaskPack<VEC> ok[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) p[u] = next[u];
-      const uint32_t ok = next_ok;
-      if (block + q + 1 < r1) load(block + q + 1);
-      const ColumnRow<A> k = rows[q];
-      if (k.u == (A)0) continue;
+      for (int u = 0; u < U; ++u) {
+        p[u] = next[u];
+        ok[u] = next_mask[u];
+      }
+      if (q + 1 < count && j0 < kn.n) load(block + q + 1);
+      if (j0 >= k.n) continue;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const A v = to_acc(p[e / VEC].v[e % VEC]);
         const A w = k.u * exp2_acc((v - k.m) * k.c - k.log2s);
-        const bool in = place(e) < k.n && ((ok >> e) & 1) && v != neg_inf<A>();
+        const bool in = off[e / VEC] + e % VEC < k.n && (!mask || ok[e / VEC].v[e % VEC]) && v != neg_inf<A>();
         acc[e] += in ? w : (A)0;
       }
     }
   }
 #pragma unroll
-  for (int u = 0; u < U; ++u) store_sums<A, VEC>(a, b, blockIdx.y, j0 + u * SPAN + mine, acc + u * VEC);
+  for (int u = 0; u < U; ++u) store_sums<A, VEC>(a, b, blockIdx.y, j0 + u * SPAN + (int)threadIdx.x * VEC, off[u], acc + u * VEC);
 }
 
 // decay w + the groups' partial sums in their order: 64 candidates per workgroup, the groups dealt to its four waves
@@ -921,14 +948,13 @@ WeightPlan weight_plan(int64_t pools, int64_t R, int64_t M, int dtype) {
   }
   return WeightPlan{false, 4, 1};
 }
-int column_groups(int64_t pools, int64_t R, int64_t M, int vec) {
-  const int64_t tile = 256 * vec * COL_VECS, tiles = (M + tile - 1) / tile * (pools > 0 ? pools : 1);
+int column_groups(int64_t pools, int64_t R, int64_t M, int dtype) {
+  const int64_t tile = 256 * (dtype == GPX_DTYPE_F64 ? 4 : 8), tiles = (M + tile - 1) / tile * (pools > 0 ? pools : 1);
   int64_t g = (1024 + tiles - 1) / tiles; // workgroups that keep the memory busy
   const int64_t most = (R + 15) / 16;
   g = g > most ? most : g;
   return (int)(g < 1 ? 1 : (g > 64 ? 64 : g));
 }
-int vec_of(int dtype) { return dtype == GPX_DTYPE_F64 ? 2 : dtype == GPX_DTYPE_F32 ? 4 : 8; }
 int acc_of(int dtype) { return dtype == GPX_DTYPE_F64 ? 8 : 4; }
 
 struct WeightSpace {
@@ -936,7 +962,7 @@ struct WeightSpace {
 };
 WeightSpace weight_space(int64_t pools, int64_t R, int64_t M, int dtype) {
   const WeightPlan p = weight_plan(pools, R, M, dtype);
-  const int groups = p.one_pass ? p.groups : column_groups(pools, R, M, vec_of(dtype));
+  const int groups = p.one_pass ? p.groups : column_groups(pools, R, M, dtype);
   WeightSpace s{};
   s.part = groups > 1 ? round_up64(pools * groups * M * acc_of(dtype), 256) : 0;
   if (!p.one_pass) {
@@ -959,9 +985,13 @@ void weights_launch(const WeightArgs& a, const WeightPlan& p, int64_t pools, hip
     else
       hipLaunchKernelGGL((pool_weights_kernel<T, sizeof(T) == 8 ? 8 : 16, 1>), grid, dim3(p.waves * 64), 0, st, a);
   } else {
-    const int tile = 256 * VecOf<T>::value * COL_VECS;
+    const int tile = 256 * VecOf<T>::value * col_vecs(sizeof(T));
     const unsigned tiles = (unsigned)((a.sc.M + tile - 1) / tile);
-    hipLaunchKernelGGL(pool_columns_kernel<T>, dim3(tiles, a.groups, (unsigned)pools), dim3(256), 0, st, a);
+    const dim3 grid(tiles, a.groups, (unsigned)pools);
+    if (a.sc.xc == 1 && (!a.sc.mask || a.sc.mc == 1))
+      hipLaunchKernelGGL((pool_columns_kernel<T, true>), grid, dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((pool_columns_kernel<T, false>), grid, dim3(256), 0, st, a);
   }
   if (a.groups > 1) hipLaunchKernelGGL(pool_weights_join_kernel<A>, dim3((a.sc.M + 63) / 64, (unsigned)pools), dim3(256), 0, st, a);
 }
@@ -1033,7 +1063,7 @@ int gpx_pool_weights(gpx_ctx* ctx, const gpx_scores* scores, const void* d_row_w
   a.parts = static_cast<char*>(d_workspace) + s.part + s.stats;
   a.splits = 1;
   a.decay = decay;
-  a.groups = p.one_pass ? p.groups : column_groups(scores->pools, a.sc.R, a.sc.M, vec_of(scores->dtype));
+  a.groups = p.one_pass ? p.groups : column_groups(scores->pools, a.sc.R, a.sc.M, scores->dtype);
   DeviceGuard g(ctx->device);
   GPX_HIP(ctx, g.err);
   hipStream_t st = static_cast<hipStream_t>(stream);
