@@ -114,8 +114,8 @@ class _Device:
             raise ValueError(f"{name} has dtype {a.dtype}; expected {' or '.join(kinds)}")
         if a.requires_grad and _torch.is_grad_enabled():
             raise ValueError(f"{name} requires grad, and no graph is recorded: detach it and call choice_logprobs_grad")
-        if a.is_neg():
-            a = a.resolve_neg()
+        if a.is_neg() or a.is_conj():
+            a = a.resolve_conj().resolve_neg()
         return a.contiguous() if contiguous else a
 
     def kind(self, a) -> str:
@@ -136,6 +136,17 @@ class _Device:
     def room(self, nbytes: int):
         return self.ref.new_empty(nbytes, dtype=_type_of["uint8"]) if nbytes else None
 
+    def write_to(self, a, *others) -> None:
+        """`a` is a result in the caller's memory: nothing else that the call reads may lie there."""
+        start, end = _extent(a)
+        for o in others:
+            if o is not None:
+                s, e = _extent(o)
+                if s < end and start < e:
+                    raise ValueError("out overlaps another argument")
+        if not a.is_inference():
+            _torch.autograd.graph.increment_version(a)
+
     def run(self, inputs, outputs, fn, room=None) -> None:
         with self.engine._pool_lock:
             fn(self.engine, _address, _stream_of(self.index))
@@ -143,6 +154,14 @@ class _Device:
 
 def _address(a) -> int:
     return 0 if a is None else a.data_ptr()
+
+
+def _extent(a):
+    """Addresses from the first to behind the last element of a tensor."""
+    start = a.data_ptr()
+    if a.numel() == 0:
+        return start, start
+    return start, start + (sum((n - 1) * s for n, s in zip(a.shape, a.stride())) + 1) * a.element_size()
 
 
 class _Room(NamedTuple):
@@ -210,7 +229,7 @@ def _broadcast_strides(shape, strides, to, name: str):
     """Strides that read an array of `shape` as one of shape `to`."""
     if shape == to:
         return strides
-    if len(shape) == 1 and shape[0] == to[-1]:
+    if len(shape) == 1 and to and shape[0] == to[-1]:
         return (0,) * (len(to) - 1) + strides
     lead = len(to) - len(shape)
     out = [0] * len(to)
@@ -320,15 +339,17 @@ def choice_logprobs(scores, choices=None, *, temperature=1.0, mask=None, lengths
         choices: the candidates whose log probabilities are wanted, shape scores.shape[:-1] (one a row) or
             scores.shape[:-1] + (C,); -1 is a filler (log probability 0), a candidate that does not exist has -inf
             (a number outside the pool: ValueError for NumPy arrays, NaN for tensors)
-        temperature: T, a number or an array broadcast to the rows (of the accumulator's type)
+        temperature: T, a number or an array broadcast to the rows (of the accumulator's type); positive and finite
+            (anything else: ValueError for numbers and NumPy arrays, a row of NaN for tensors)
         mask: which candidates may be chosen, bool or uint8, broadcast to the scores
         lengths: how many candidates each row has, int64 or int32, broadcast to the rows (clamped to 0 .. M)
         top: number of best alternatives to return, at most 64
 
     Returns:
         ChoiceLogprobs: logprobs (as choices; None without them), entropy and logsumexp (one a row), top_indices and
-        top_logprobs (rows, top; None for top = 0): score descending, equal scores by index, -1 and -inf where fewer exist; a row in which nothing exists has entropy 0
-        and logsumexp -inf; a row with a NaN or +inf among what exists is NaN (NaN scores are never alternatives)
+        top_logprobs (rows, top; None for top = 0): score descending, equal scores by index, -1 and -inf where fewer exist;
+        a row in which nothing exists has entropy 0 and logsumexp -inf; a row with a NaN or +inf among what exists is NaN
+        (NaN scores are never alternatives)
     """
     pol = _Policy(scores, temperature, mask, lengths)
     top = int(top)
@@ -424,7 +445,7 @@ def pool_weights(scores, weights=None, *, decay: float = 1.0, row_weights=None, 
         decay: factor on them, finite and not negative; 0 forgets them, whatever they are
         row_weights: factor of each row, of the accumulator's type, shape scores.shape[:-1]; a row of weight 0 is not read
         temperature, mask, lengths: as for choice_logprobs
-        out: array for the result (may be `weights`)
+        out: array for the result; may be `weights`, and may not overlap any other argument
 
     Returns:
         the new weights, (M,) or (pools, M).  A row in which nothing exists adds nothing; a NaN row makes what exists in it
@@ -450,11 +471,13 @@ def pool_weights(scores, weights=None, *, decay: float = 1.0, row_weights=None, 
     if out is None:
         res = sp.new(shape, pol.acc)
     else:
-        res = sp.take(out, "out", (pol.acc,)) if not sp.host else out
-        ok = tuple(res.shape) == shape and (res.is_contiguous() if not sp.host else
-                                            res.flags.c_contiguous and res.flags.writeable and res.dtype.name == pol.acc)
+        res = out if sp.host else sp.take(out, "out", (pol.acc,))
+        ok = tuple(res.shape) == shape and (res.flags.c_contiguous and res.flags.writeable and res.dtype.name == pol.acc and
+                                            res.dtype.isnative if sp.host else res is out and res.is_contiguous())
         if not ok:
             raise ValueError(f"out must be contiguous, of shape {shape} and of type {pol.acc}")
+        if not sp.host:
+            sp.write_to(res, *pol.inputs(), u, None if w is None or w.data_ptr() == res.data_ptr() else w)
     nbytes = _weights_workspace(pol.pools, pol.rows, pol.M, _DTYPES[pol.kind])
     ws = sp.room(nbytes)
 

@@ -201,7 +201,7 @@ struct Waiting {
     A bound = shared;
     const bool many = __popcll(better) >= (list.k > 32 ? list.k : 32);
     if (many) {
-      A sorted = cm;
+      A sorted = cm == cm ? cm : neg_inf<A>(); // (a lane of NaN scores only: the network would lose another lane's)
       bitonic_values<2, 1>(sorted);
       A kth = read_lane(sorted, list.k - 1);
       if (TWO && list.k > TWO_PER_LANE) {
@@ -589,8 +589,8 @@ int pool_scores_view(gpx_ctx* ctx, const gpx_scores* x, PoolScores* out, const c
   if (!x) return no("null scores");
   if (x->dtype < GPX_DTYPE_F64 || x->dtype > GPX_DTYPE_F16) return no("dtype");
   if (x->pools < 0 || x->rows < 0 || x->candidates < 0) return no("negative size");
-  if (x->candidates > INT32_MAX - (1 << 20)) return no("more than 2^31 - 2^20 candidates");
-  if (x->rows > 0 && x->pools > (int64_t)(1 << 25) / x->rows) return no("more than 2^25 rows");
+  if (x->candidates > POOL_MAX) return no("more than 2^31 - 2^20 candidates");
+  if (!pool_sizes_hold(x->pools, x->rows, x->candidates)) return no("more than 2^25 rows");
   if (x->pools * x->rows > 0 && x->candidates > 0 && !x->d_scores) return no("null scores");
   if (!x->d_temperatures && !(x->temperature > 0 && x->temperature < INFINITY)) return no("the temperature must be positive and finite");
   out->x = x->d_scores;
@@ -634,7 +634,7 @@ int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, void* d_stat
 extern "C" {
 
 int64_t gpx_choice_workspace(int64_t pools, int64_t rows, int64_t candidates, int dtype, int top) {
-  if (pools < 0 || rows < 0 || candidates < 0 || top < 0 || top > TOP_MAX || dtype < GPX_DTYPE_F64 || dtype > GPX_DTYPE_F16) return -1;
+  if (!pool_sizes_hold(pools, rows, candidates) || top < 0 || top > TOP_MAX || dtype < GPX_DTYPE_F64 || dtype > GPX_DTYPE_F16) return -1;
   return choice_workspace(pools * rows, candidates, dtype, top);
 }
 

@@ -377,6 +377,10 @@ __device__ __forceinline__ void row_reference(const void* stats, const void* par
 }
 
 // pool.hip / choice.hip, host side
+constexpr int64_t POOL_MAX = INT32_MAX - (1 << 20), ROWS_MAX = 1 << 25; // candidates of a pool; rows of all pools
+inline bool pool_sizes_hold(int64_t pools, int64_t rows, int64_t candidates) {
+  return pools >= 0 && rows >= 0 && candidates >= 0 && candidates <= POOL_MAX && (rows == 0 || pools <= ROWS_MAX / rows);
+}
 int pool_scores_view(gpx_ctx* ctx, const gpx_scores* x, PoolScores* out, const char* what);
 struct DeviceGuard { // the caller's current device comes back whatever happens
   int before = -1;

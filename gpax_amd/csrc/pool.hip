@@ -434,19 +434,20 @@ __device__ __forceinline__ void move_rows(char* dst, const char* s0, const char*
 // candidates j0 + kept[0 .. count) of pool b become those that stay from place pos0 on
 template <typename W>
 __device__ __forceinline__ void put_kept(const EvictArgs& a, int64_t b, int64_t pos0, int64_t j0, const uint16_t* kept, int count) {
-  for (int p0 = threadIdx.x; p0 < count; p0 += PUT * 1024) {
-    const int n = (count - p0 + 1023) / 1024; // of this lane's, at most PUT are moved now
+  constexpr int T = 1024; // threads
+  for (int p0 = threadIdx.x; p0 < count; p0 += PUT * T) {
+    const int n = (count - p0 + T - 1) / T; // of this lane's, at most PUT are moved now
     const int64_t at = b * a.K + pos0 + p0;
-    const int64_t j_0 = j0 + kept[p0], j_1 = n > 1 ? j0 + kept[p0 + 1024] : j_0;
-    const int64_t j_2 = n > 2 ? j0 + kept[p0 + 2048] : j_0, j_3 = n > 3 ? j0 + kept[p0 + 3072] : j_0;
+    const int64_t j_0 = j0 + kept[p0], j_1 = n > 1 ? j0 + kept[p0 + T] : j_0;
+    const int64_t j_2 = n > 2 ? j0 + kept[p0 + 2 * T] : j_0, j_3 = n > 3 ? j0 + kept[p0 + 3 * T] : j_0;
     const W* w = static_cast<const W*>(a.weights) + b * a.M;
     W* out = static_cast<W*>(a.out) + at;
     const W w0 = w[j_0], w1 = w[j_1], w2 = w[j_2], w3 = w[j_3];
     a.indices[at] = j_0;
     out[0] = w0;
-    if (n > 1) a.indices[at + 1024] = j_1, out[1024] = w1;
-    if (n > 2) a.indices[at + 2048] = j_2, out[2048] = w2;
-    if (n > 3) a.indices[at + 3072] = j_3, out[3072] = w3;
+    if (n > 1) a.indices[at + T] = j_1, out[T] = w1;
+    if (n > 2) a.indices[at + 2 * T] = j_2, out[2 * T] = w2;
+    if (n > 3) a.indices[at + 3 * T] = j_3, out[3 * T] = w3;
     for (int y = 0; y < a.npay; ++y) {
       const int64_t bytes = a.pay[y].bytes;
       const char* s = a.pay[y].src + b * a.M * bytes;
@@ -1033,12 +1034,12 @@ void evict_launch(const EvictArgs& a, int64_t pools, hipStream_t st) {
 extern "C" {
 
 int64_t gpx_pool_evict_workspace(int64_t pools, int64_t candidates, int dtype) {
-  if (pools < 0 || candidates < 0 || (dtype != GPX_DTYPE_F64 && dtype != GPX_DTYPE_F32)) return -1;
+  if (pools < 0 || pools > 65535 || candidates < 0 || candidates > POOL_MAX || (dtype != GPX_DTYPE_F64 && dtype != GPX_DTYPE_F32)) return -1;
   return evict_workspace(dtype, pools, candidates);
 }
 
 int64_t gpx_pool_weights_workspace(int64_t pools, int64_t rows, int64_t candidates, int dtype) {
-  if (pools < 0 || rows < 0 || candidates < 0 || dtype < GPX_DTYPE_F64 || dtype > GPX_DTYPE_F16) return -1;
+  if (!pool_sizes_hold(pools, rows, candidates) || pools > 65535 || dtype < GPX_DTYPE_F64 || dtype > GPX_DTYPE_F16) return -1;
   return weight_space(pools, rows, candidates, dtype).total;
 }
 
@@ -1086,10 +1087,10 @@ int gpx_pool_evict(gpx_ctx* ctx, int dtype, int64_t pools, int64_t candidates, c
                    void* stream) {
   if (!ctx || ctx->device < 0) return -1;
   if (dtype != GPX_DTYPE_F64 && dtype != GPX_DTYPE_F32) return bad_arg(ctx, "gpx_pool_evict: weights are float64 or float32");
-  if (pools < 0 || candidates < 0 || pools > 65535 || candidates > INT32_MAX - (1 << 20))
+  if (pools < 0 || candidates < 0 || pools > 65535 || candidates > POOL_MAX)
     return bad_arg(ctx, "gpx_pool_evict: sizes");
   if (budget < 1 || budget > INT32_MAX) return bad_arg(ctx, "gpx_pool_evict: the budget must be positive");
-  if (first < 0 || recent < 0 || first + recent > budget) return bad_arg(ctx, "gpx_pool_evict: first + recent exceed the budget");
+  if (first < 0 || recent < 0 || first > budget || recent > budget - first) return bad_arg(ctx, "gpx_pool_evict: first + recent exceed the budget");
   if (npayload < 0 || npayload > 16) return bad_arg(ctx, "gpx_pool_evict: at most 16 payload arrays");
   if (pools == 0) return 0;
   if ((!d_weights && candidates > 0) || !d_indices || !d_new_lengths || !d_weights_out) return bad_arg(ctx, "gpx_pool_evict: null pointer");

@@ -494,3 +494,48 @@ def test_the_library_refuses_what_the_kernels_do_not_take():
         eng.pool_evict(0, 1, 8, 0, 0, False, 0, 4, 0, 0, 1, 1, 1, [], [], [], 0, 0, 0)
     with pytest.raises(_lib.GpxError):  # needs a workspace
         eng.pool_evict(0, 1, 1 << 20, 1, 0, False, 0, 4, 0, 0, 1, 1, 1, [], [], [], 0, 0, 0)
+    for first, recent in [(1 << 62, 1 << 62), (5, 0), (0, 5), (4, 1)]:
+        with pytest.raises(_lib.GpxError):
+            eng.pool_evict(0, 1, 8, 1, 0, False, 0, 4, first, recent, 1, 1, 1, [], [], [], 0, 0, 0)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("M", [1024, 5000, 70001])
+def test_alternatives_beside_nan_scores(kind, M):
+    """NaN scores are never alternatives, and hide none: lanes that meet nothing else, a few places, nearly all of them."""
+    rng = np.random.default_rng(M)
+    for share, top in [("lanes", 20), ("lanes", 40), ("few", 64), ("most", 30)]:
+        x = scores_of(rng, kind, (3, M))
+        if share == "lanes":  # 16 neighbours of every 64: whole vectors of some lanes
+            x[:, torch.arange(M, device="cuda") % 64 < 16] = math.nan
+        else:
+            x[torch.as_tensor(rng.random((3, M)) < (0.01 if share == "few" else 0.97), device="cuda")] = math.nan
+        r = acq.choice_logprobs(x, top=top)
+        assert torch.isnan(r.entropy).all()
+        np.testing.assert_array_equal(host(r.top_indices), ref.choice(host(x), top=top)["top_indices"])
+
+
+def test_out_lies_apart_from_what_is_read():
+    x = torch.randn(4, 64, device="cuda")
+    w = torch.randn(64, device="cuda")
+    want = acq.pool_weights(x, w, decay=0.5)
+    before = w._version
+    assert torch.equal(acq.pool_weights(x, w, decay=0.5, out=w), want) and w._version > before
+    room = torch.zeros(4, 64, device="cuda")
+    assert acq.pool_weights(x, out=room[2]).data_ptr() == room[2].data_ptr()
+    both = torch.zeros(80, device="cuda")
+    for call in [lambda: acq.pool_weights(x, out=x[1]), lambda: acq.pool_weights(x, both[:64], out=both[16:]),
+                 lambda: acq.pool_weights(x, row_weights=both[60:64], out=both[:64]), lambda: acq.pool_weights(x, temperature=both[:4] + 1, out=x[3]),
+                 lambda: acq.pool_weights(x, mask=room.view(torch.uint8)[0, :64], out=room[0])]:
+        with pytest.raises(ValueError):
+            call()
+    assert acq.pool_weights(x, both[:16].new_zeros(64), out=both[:64]).data_ptr() == both.data_ptr()
+
+
+def test_lazily_conjugated_and_negated_payload():
+    z = torch.randn(9, 3, dtype=torch.complex64, device="cuda")
+    w = torch.randn(9, device="cuda")
+    for rows in (z.conj(), z.conj().imag):
+        r = acq.pool_evict(w, 4, (rows,))
+        assert torch.equal(r.payload[0], rows[r.indices])
+    assert torch.equal(acq.pool_evict(z[:, 0].conj().imag, 4).weights, z[:, 0].conj().imag[acq.pool_evict(-z[:, 0].imag, 4).indices])

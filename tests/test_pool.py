@@ -168,6 +168,9 @@ BAD = {
     "budget": lambda: acq.pool_evict(X, 0), "protected": lambda: acq.pool_evict(X, 4, first=3, recent=2), "negative": lambda: acq.pool_evict(X, 4, recent=-1),
     "weights of three dimensions": lambda: acq.pool_evict(X[None], 4), "payload shape": lambda: acq.pool_evict(X, 4, (np.zeros((3, 9)),)),
     "many payloads": lambda: acq.pool_evict(X, 4, (X,) * 17), "payload type": lambda: acq.pool_evict(X, 4, (np.full((3, 10), "a"),)),
+    "lengths of a row that is none of several": lambda: acq.choice_logprobs(X[0], lengths=np.ones(1, np.int64)),
+    "temperatures of a row that is none of several": lambda: acq.pool_weights(X[0], temperature=np.ones(1)),
+    "out read-only": lambda: acq.pool_weights(X, out=np.broadcast_to(np.zeros(10), (10,))),
     "lengths of pools": lambda: acq.pool_evict(X, 4, lengths=np.ones(2, np.int64)),
 }
 
@@ -204,6 +207,11 @@ def test_workspace_sizes_come_from_sizes_alone():
     assert lib.gpx_choice_workspace(1, -1, 4, 0, 0) < 0 and lib.gpx_choice_workspace(1, 1, 4, 9, 0) < 0 and lib.gpx_choice_workspace(1, 1, 4, 0, 65) < 0
     assert lib.gpx_pool_weights_workspace(1, 1, 10, 0) == 0 and lib.gpx_pool_weights_workspace(1, 1000, 1024, 0) > 0
     assert lib.gpx_pool_weights_workspace(-1, 1, 1, 0) < 0
+    # sizes that the operators refuse have none (2^31 - 2^20 candidates, 2^25 rows, 65535 pools)
+    assert lib.gpx_choice_workspace(1, 1, (1 << 31) - (1 << 20), 0, 1) < 0 and lib.gpx_choice_workspace(1 << 40, 1 << 40, 4, 0, 1) < 0
+    assert lib.gpx_pool_weights_workspace(1 << 16, 1, 4, 0) < 0 and lib.gpx_pool_weights_workspace(1 << 13, 1 << 13, 4, 0) < 0
+    assert lib.gpx_pool_evict_workspace(1 << 16, 4, 0) < 0 and lib.gpx_pool_evict_workspace(1, 1 << 31, 0) < 0
+    assert lib.gpx_pool_evict_workspace(2, 16384, 0) == 0 and lib.gpx_pool_evict_workspace(2, 16385, 1) > 0
 
 
 @pytest.mark.parametrize("source", ["choice.hip", "pool.hip"])
