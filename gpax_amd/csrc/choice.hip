@@ -17,7 +17,7 @@ using namespace gpx;
 namespace {
 
 constexpr int TOP_MAX = 64;    // alternatives per row: one per lane of a wave
-constexpr int TWO_PER_LANE = 24; // lists longer than this: see Waiting::step (8 x 262144 float64 top 64: 26 -> 16 us)
+constexpr int LONG_LIST = 24;  // more alternatives than this: thresholds from 128 or 256 instead of 64 maxima
 constexpr int INSERT_MAX = 10; // more than this many newcomers in one vector: sort and merge instead of inserting one by one
 
 struct ChoiceArgs {
@@ -74,6 +74,7 @@ __device__ __forceinline__ void bitonic(A& k, uint32_t& i) {
   else if constexpr (SIZE < 64)
     bitonic<SIZE * 2, SIZE>(k, i);
 }
+
 template <int SIZE, int STRIDE, typename A>
 __device__ __forceinline__ void bitonic_values(A& v) {
   constexpr uint64_t KEEP = keep_better(SIZE, STRIDE);
@@ -83,6 +84,70 @@ __device__ __forceinline__ void bitonic_values(A& v) {
     bitonic_values<SIZE, STRIDE / 2>(v);
   else if constexpr (SIZE < 64)
     bitonic_values<SIZE * 2, SIZE>(v);
+}
+// The k-th largest of the wave's 64 V values (no NaN), or a little less; -inf if fewer than k exist.  64 values are sorted (21
+// exchanges).  More are not moved: it is found bit by bit in integers of their order, from the top, with a comparison a value
+// and the counting in the scalar unit; a prefix that exactly k reach ends it.  (Of 64 values that takes longer: 65536 x 1024
+// bfloat16 top 8 80 instead of 72 us; of 128, 39 us against 57 for 512 x 65536 float32 top 64.)
+__device__ __forceinline__ uint32_t order_word(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ uint32_t order_word(double v) { // (64 bits: of the high word)
+  const uint32_t u = (uint32_t)__double2hiint(v);
+  return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float least_of_order(uint32_t t, float) {
+  return t <= 0x007fffffu ? neg_inf<float>() : __uint_as_float((t >> 31) ? t & 0x7fffffffu : ~t);
+}
+__device__ __forceinline__ uint32_t low_order(double v) {
+  const uint32_t u = (uint32_t)__double2loint(v);
+  return __double2hiint(v) < 0 ? ~u : u;
+}
+template <typename A, int V>
+__device__ __forceinline__ A kth_of(const A (&v)[V], int k) {
+  if constexpr (V == 1) {
+    A sorted = v[0];
+    bitonic_values<2, 1>(sorted);
+    return read_lane(sorted, k - 1);
+  }
+  uint32_t w[V], t = 0;
+  int reach = 64 * V; // how many are at least t
+#pragma unroll
+  for (int i = 0; i < V; ++i) w[i] = order_word(v[i]);
+#pragma unroll 1
+  for (uint32_t bit = 1u << 31; bit != 0 && reach != k; bit >>= 1) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) c += __popcll(__ballot(w[i] >= (t | bit)));
+    if (c >= k) {
+      t |= bit;
+      reach = c;
+    }
+  }
+  if constexpr (sizeof(A) == 4) {
+    return least_of_order(t, 0.0f);
+  } else {
+    if (t <= 0x000fffffu) return neg_inf<A>();
+    const uint32_t hi = (t >> 31) ? t & 0x7fffffffu : ~t;
+    uint32_t low = 0;
+    if (reach > k + 4) { // values that agree in 32 bits: the same for the low word
+      uint32_t l[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) l[i] = low_order(v[i]);
+#pragma unroll 1
+      for (uint32_t bit = 1u << 31; bit != 0 && reach != k; bit >>= 1) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) c += __popcll(__ballot(w[i] > t || (w[i] == t && l[i] >= (low | bit))));
+        if (c >= k) {
+          low |= bit;
+          reach = c;
+        }
+      }
+    }
+    return __hiloint2double((int)hi, (int)((t >> 31) ? low : ~low));
+  }
 }
 
 template <typename A>
@@ -165,11 +230,10 @@ struct WaitingRoom {
   A keys[64];
   uint32_t idx[64 * E + 64];
 };
-// TWO: for lists longer than TWO_PER_LANE, a better bound (where registers allow it: not for 16-bit scores, which need eight
-// waves a SIMD, nor for 64-bit ones in workgroups of 16 waves)
-template <typename T, int VEC, int U, bool TWO>
+template <typename T, int VEC, int U>
 struct Waiting {
   typedef typename Acc<T>::type A;
+  static constexpr int GROUP = sizeof(A) == 4 ? 4 : U * VEC; // (of 64 bits the groups' maxima would not fit the registers)
   WaitingRoom<A, U * VEC>& room; // this wave's
   A shared;                      // k candidates of the row reach it
   int count;
@@ -201,37 +265,44 @@ struct Waiting {
     A bound = shared;
     const bool many = __popcll(better) >= (list.k > 32 ? list.k : 32);
     if (many) {
-      A sorted = cm == cm ? cm : neg_inf<A>(); // (a lane of NaN scores only: the network would lose another lane's)
-      bitonic_values<2, 1>(sorted);
-      A kth = read_lane(sorted, list.k - 1);
-      if (TWO && list.k > TWO_PER_LANE) {
-        // for a long list the lanes' next best count too: of two sorted lists the larger of (a_i, b_63-i) are the best 64 of
-        // both; sorted again, the k-th of them.  (One score after the other: as a tree it takes twice the registers.)
-        A m2 = neg_inf<A>();
+      A kth;
+      if (list.k <= LONG_LIST) {
+        const A top[1] = {cm == cm ? cm : neg_inf<A>()}; // (NaN: nothing else in this lane)
+        kth = kth_of(top, list.k);
+      } else { // so many of 64 maxima would be too low a bound: four to a lane
+        constexpr int Q = U * VEC / 4;
+        A top[4];
 #pragma unroll
-        for (int e = 0; e < U * VEC; ++e) {
-          m2 = fmax(m2, x[e] < cm ? x[e] : m2);
-          asm volatile("" : "+v"(m2));
+        for (int q = 0; q < 4; ++q) {
+          top[q] = neg_inf<A>();
+#pragma unroll
+          for (int e = q * Q; e < (q + 1) * Q; ++e) top[q] = fmax(top[q], x[e]);
         }
-        bitonic_values<2, 1>(m2);
-        m2 = __shfl(m2, 63 - lane);
-        sorted = fmax(sorted, m2);
-        bitonic_values<64, 32>(sorted);
-        kth = read_lane(sorted, list.k - 1);
+        kth = kth_of(top, list.k);
       }
       bound = kth > bound ? kth : bound;
     }
+    // four scores at a time: most steps hold one or two that pass, and the other groups are left with one comparison
 #pragma unroll
-    for (int e = 0; e < U * VEC; ++e) {
-      const bool in = x[e] > own && x[e] >= bound;
-      const uint64_t mask = __ballot(in);
-      if (mask) {
-        const int at = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
-        if (in) {
-          room.idx[at] = (uint32_t)(j0 + (e / VEC) * 64 * VEC + lane * VEC + e % VEC);
-          if (at < 64) room.keys[at] = x[e];
+    for (int g = 0; g < U * VEC; g += GROUP) {
+      if (GROUP < U * VEC) {
+        A gm = x[g];
+#pragma unroll
+        for (int e = g + 1; e < g + GROUP; ++e) gm = fmax(gm, x[e]);
+        if (__ballot(gm > own && gm >= bound) == 0) continue;
+      }
+#pragma unroll
+      for (int e = g; e < g + GROUP; ++e) {
+        const bool in = x[e] > own && x[e] >= bound;
+        const uint64_t mask = __ballot(in);
+        if (mask) {
+          const int at = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+          if (in) {
+            room.idx[at] = (uint32_t)(j0 + (e / VEC) * 64 * VEC + lane * VEC + e % VEC);
+            if (at < 64) room.keys[at] = x[e];
+          }
+          count += __popcll(mask);
         }
-        count += __popcll(mask);
       }
     }
     if (many || count >= 64) flush(list, v, lane); // (many: the threshold will be much better)
@@ -243,22 +314,25 @@ struct Waiting {
 template <typename A, int W>
 struct WaveShare {
   Stats<A> st[W];
-  A thr;
+  A cells[W > 1 ? 2 : 1][W > 1 ? 128 : 1]; // two in turn: all waves have read one when they meet over the other
 };
-// The k-th best of all waves' candidates so far.  Lists stay with their waves.
-template <typename A, int W, int E>
-__device__ __forceinline__ A common_threshold(const TopList<A>& list, WaitingRoom<A, E>* rooms, WaveShare<A, W>& sh, int wave, int lane) {
-  rooms[wave].keys[lane] = list.key;
-  rooms[wave].idx[lane] = list.idx;
+// A threshold for all waves: the k-th largest of 64 (for long lists 128) maxima, each over all that some lanes of one wave have
+// met, so that k candidates of the row reach it.  (Merging the waves' lists for it, one after the other in one wave while the
+// others waited, let fewer pass and cost three times as much: 512 x 65536 float32 top 20 took 67 us.)
+template <int CELLS, typename A, int W>
+__device__ __forceinline__ A common_threshold(A most, int k, WaveShare<A, W>& sh, int turn, int wave, int lane) {
+  constexpr int LANES = 64 * W / CELLS; // of a cell
+  if constexpr (LANES > 1) most = fmax(most, xor_lane<1>(most));
+  if constexpr (LANES > 2) most = fmax(most, xor_lane<2>(most));
+  if constexpr (LANES > 4) most = fmax(most, xor_lane<4>(most));
+  if constexpr (LANES > 8) most = fmax(most, xor_lane<8>(most));
+  static_assert(LANES >= 1 && LANES <= 16, "xor over 16 lanes");
+  if (lane % LANES == 0) sh.cells[turn][wave * (64 / LANES) + lane / LANES] = most;
   __syncthreads();
-  if (wave == 0) {
-    TopList<A> all = list;
-#pragma unroll 1
-    for (int w = 1; w < W; ++w) all.consume_sorted(rooms[w].keys[lane], rooms[w].idx[lane], lane);
-    if (lane == 0) sh.thr = all.thr_key;
-  }
-  __syncthreads();
-  return sh.thr;
+  A top[CELLS / 64];
+#pragma unroll
+  for (int i = 0; i < CELLS / 64; ++i) top[i] = sh.cells[turn][i * 64 + lane];
+  return kth_of(top, k);
 }
 
 // What a row's statistics are turned into, by a team of `size` threads of which this one is `at`; the list by its wave.
@@ -346,25 +420,30 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, sizeof(T) == 8 || WA
   const int first = WAVES == 1 ? 0 : ((int)blockIdx.y * WAVES + wave) * step;
   const int stride = WAVES == 1 ? step : a.splits * WAVES * step;
   const int steps = (int)(((uint32_t)v.n + (uint32_t)stride - 1) / (uint32_t)stride); // the same for all waves of the row's workgroup: they meet at barriers
-  Waiting<T, VEC, U, (sizeof(T) == 4 || (sizeof(T) == 8 && WAVES != 16))> waiting{sh_room[TOP ? wave : 0], neg_inf<A>(), 0};
+  Waiting<T, VEC, U> waiting{sh_room[TOP ? wave : 0], neg_inf<A>(), 0};
+  A most = neg_inf<A>(); // that this lane has met
+  int turn = 0;
   for (int i = 0; i < steps; ++i) {
     const int j0 = first + i * stride;
+    A x[U * VEC], cm = neg_inf<A>();
     if (j0 < v.n) {
-      A x[U * VEC];
       load_step<T, VEC, U>(v, j0, 64 * VEC, lane * VEC, x);
-      A cm = x[0];
+      cm = x[0];
 #pragma unroll
       for (int e = 1; e < U * VEC; ++e) cm = fmax(cm, x[e]);
       stats_add<A, U * VEC>(st, x, cm, c);
-      if constexpr (TOP) waiting.step(list, v, x, cm, j0, lane);
     }
     if constexpr (TOP && WAVES > 1) {
-      // a threshold of the whole row after 1, 2, 4 ... steps: between two of them about k candidates of the row pass it
-      if (i + 1 < steps && ((i + 1) & i) == 0) {
-        waiting.flush(list, v, lane);
-        waiting.shared = common_threshold(list, sh_room, sh_share, wave, lane);
+      // a threshold of the whole row at steps 1, 2, 4 ...: between two of them about k candidates of the row pass it
+      most = fmax(most, cm);
+      if (((i + 1) & i) == 0) {
+        waiting.shared = list.k <= LONG_LIST ? common_threshold<64>(most, list.k, sh_share, turn, wave, lane)
+                                             : common_threshold<128>(most, list.k, sh_share, turn, wave, lane);
+        turn ^= 1;
       }
     }
+    if constexpr (TOP)
+      if (j0 < v.n) waiting.step(list, v, x, cm, j0, lane);
   }
   if constexpr (TOP) waiting.flush(list, v, lane);
   st = stats_wave(st, c);

@@ -539,3 +539,19 @@ def test_lazily_conjugated_and_negated_payload():
         r = acq.pool_evict(w, 4, (rows,))
         assert torch.equal(r.payload[0], rows[r.indices])
     assert torch.equal(acq.pool_evict(z[:, 0].conj().imag, 4).weights, z[:, 0].conj().imag[acq.pool_evict(-z[:, 0].imag, 4).indices])
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("shape", [(3, 1024), (2, 5000), (2, 70001)], ids=str)
+def test_alternatives_of_scores_that_lie_close_together(kind, shape, sign):
+    """Scores that differ in their last bits only, around a large value of either sign, many of them equal; and rows that rise or
+    fall all along, so that every step passes every threshold or none does."""
+    rng = np.random.default_rng(shape[1])
+    step = {"float64": 1e-12, "float32": 1e-3, "bfloat16": 8.0, "float16": 1.0}[kind]
+    near = torch.as_tensor(sign * (1000.0 + step * rng.standard_normal(shape)), device="cuda").to(getattr(torch, kind))
+    ramp = torch.linspace(-50, 50, shape[1], device="cuda", dtype=torch.float64).expand(shape).to(getattr(torch, kind)) * sign
+    for x in (near, ramp):
+        for top in (1, 20, 25, 64):
+            r = acq.choice_logprobs(x, top=top)
+            np.testing.assert_array_equal(host(r.top_indices), ref.choice(host(x), top=top)["top_indices"])
