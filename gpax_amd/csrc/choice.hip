@@ -216,6 +216,12 @@ struct TopList {
   // a list that is sorted already
   __device__ __forceinline__ void consume_sorted(A ck, uint32_t ci, int lane) {
     if (__ballot(before(ck, ci, thr_key, thr_idx)) == 0) return;
+    if (read_lane(idx, 0) == 0xffffffffu) { // the first one
+      key = ck;
+      idx = ci;
+      rethreshold();
+      return;
+    }
     merge_sorted(ck, ci, lane);
   }
 };
@@ -223,7 +229,7 @@ struct TopList {
 // The candidates that may belong into the list.  Of a step only those at or above a bound are looked at one by one: the list's
 // threshold, the threshold of all waves of the row, or, where many lanes (and at least k) hold something better, the k-th
 // largest of the lanes' maxima (k candidates reach it, so no other can be among the best k).  What passes waits in LDS until 64
-// are together or the waves compare notes; it is offered 64 at a time, the first 64 with their scores, more than that by their
+// are together; it is offered 64 at a time, the first 64 with their scores, more than that by their
 // index, and those scores are read again from the cache.  A threshold that is not up to date only lets more pass.
 template <typename A, int E>
 struct WaitingRoom {
@@ -309,8 +315,9 @@ struct Waiting {
   }
 };
 
-// What the waves of a workgroup tell each other: statistics, and their lists in the front of their waiting rooms, which are
-// empty then (LDS decides how many workgroups a CU holds).
+// What the waves of a workgroup tell each other: maxima, and at the end statistics, and their lists in the front of their waiting
+// rooms, which are empty then (LDS decides how many workgroups a CU holds: with 1 KB more for 256 maxima, 7 instead of 8 of
+// those with 4 waves, and 2048 x 65536 bfloat16 top 20 takes 81 instead of 74 us).
 template <typename A, int W>
 struct WaveShare {
   Stats<A> st[W];
@@ -604,8 +611,11 @@ __global__ __launch_bounds__(256) void choice_grad_kernel(GradArgs a) {
 
 // ---- host -------------------------------------------------------------------------------------------------------------
 
-// Waves per row (1, 4 or 16) and workgroups per row.  Enough waves to occupy the chip (TARGET), but none with less than a
-// step to do: a row shorter than that is one wave's, however few rows there are.
+// Waves per row (1, 4 or 16) and workgroups per row.  Enough waves to occupy the chip (TARGET: 16 of the 32 that a CU holds;
+// with 32, 1024 x 16384 float32 take 15.7 instead of 13.6 us, with 8, 2048 x 65536 bfloat16 62 instead of 47), but none with less than a step to do: a row shorter than that is one wave's, however few rows there are (1000 x 1024 float64
+// 5 us as one wave a row).  One workgroup a row up to 16 waves spares the second launch (4 us) and most of the lists' joining;
+// beyond that up to 64 workgroups share one, more than 32 only if their waves have two steps each (8 x 262144 float64 top 64:
+// 32 take 15.2 us and 8.7 to join, 64 take 13.7 and 11.9; 2 x 1048576 float32: 26.4 and 7.0 against 18.1 and 9.5).
 struct ChoicePlan {
   int waves, splits;
 };
@@ -618,7 +628,8 @@ ChoicePlan choice_plan(int64_t rows, int64_t M) {
   if (want <= 4) return ChoicePlan{4, 1};
   if (want <= 16) return ChoicePlan{16, 1};
   int64_t splits = (want + 3) / 4;
-  if (splits > 64) splits = 64;
+  const int64_t most = steps < 32 * 8 ? 32 : (steps > 64 * 8 ? 64 : steps / 8);
+  if (splits > most) splits = most;
   return ChoicePlan{4, (int)splits};
 }
 
