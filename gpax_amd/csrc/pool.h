@@ -289,6 +289,52 @@ __device__ __forceinline__ void load_step(const Row<T>& v, int j0, int span, int
     }
 }
 
+// The same in two halves, for a kernel that has the next row on its way while it works on one: `load` starts the loads,
+// `decode` makes the scores of them.  DENSE: candidates (and mask bytes) side by side.  Pools of VEC candidates or more.
+template <typename T, int VEC, int U, bool DENSE>
+struct RawStep {
+  typedef typename Acc<T>::type A;
+  Pack<T, VEC> p[U];
+  MaskPack<VEC> q[U];
+
+  // vectors that would cross the end of the POOL (of M candidates) read its last ones instead
+  __device__ __forceinline__ void load(const Row<T>& v, int M, int span, int lane_j) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u * span >= v.n) continue; // uniform: nothing of it exists
+      const int j = u * span + lane_j, off = j < M - VEC ? j : M - VEC;
+      if (DENSE) {
+        p[u] = *reinterpret_cast<const Pack<T, VEC>*>(v.x + (uint32_t)off);
+        if (v.mask) q[u] = *reinterpret_cast<const MaskPack<VEC>*>(v.mask + (uint32_t)off);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          p[u].v[e] = v.x[(off + e) * v.xc];
+          if (v.mask) q[u].v[e] = v.mask[(off + e) * v.mc];
+        }
+      }
+    }
+  }
+  // x[u * VEC + e] is candidate min(u * span + lane_j, M - VEC) + e
+  __device__ __forceinline__ void decode(bool masked, int n, int M, int span, int lane_j, A* x) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if ((u + 1) * span <= n && !masked) { // uniform: all of it is there
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[u * VEC + e] = to_acc(p[u].v[e]);
+        continue;
+      }
+      const int j = u * span + lane_j, off = j < M - VEC ? j : M - VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        // a candidate belongs to the lane whose own vector it lies in
+        const bool in = u * span < n && off + e >= j && off + e < n && (!masked || q[u].v[e]);
+        x[u * VEC + e] = in ? to_acc(p[u].v[e]) : neg_inf<A>();
+      }
+    }
+  }
+};
+
 // ---- running statistics of a row --------------------------------------------------------------------------------------
 template <typename A>
 struct Stats {

@@ -27,8 +27,8 @@ struct WeightArgs {
 };
 
 constexpr int PER_LANE = 16; // candidates a lane owns in the one-pass kernel
-constexpr int TEAMS = 8;     // rows at a time of a workgroup whose teams are single waves
-// the largest team: 16 sums and 16 scores of 64 bits do not fit the 128 registers that 16 waves leave each lane
+constexpr int TEAMS = 8;     // rows at a time of a workgroup in which a row is a wave's
+// the most waves for a row: 16 sums and 16 scores of 64 bits do not fit the 128 registers that 16 waves leave each lane
 inline int team_waves(int dtype) { return dtype == GPX_DTYPE_F64 ? 8 : 16; }
 
 // finished sums of candidates j .. j + VEC, of them those from `from` on: straight to the output, or to this group's partial sums
@@ -48,37 +48,30 @@ __device__ __forceinline__ void store_sums(const WeightArgs& a, int64_t b, int g
   }
 }
 
-// One pass: a team of WAVES waves per row, NTEAMS teams per workgroup.
-template <typename T, int WAVES, int NTEAMS>
-__global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(WeightArgs a) {
+// One pass over pools of at most 1024 candidates: a row a wave, TEAMS waves per workgroup, no barrier before the end.  Bound by
+// the latency of a row or two per wave: 1000 x 1024 float64 take 8.5 us and 4.7 to join (8.2 MB, 1 TB/s), 4000 x 1024 float32
+// 7.2 and 8.4; four waves a row take 13.1 and 6.3, 16.2 and 13.4.
+template <typename T>
+__global__ __launch_bounds__(TEAMS * 64) void pool_weights_wave_kernel(WeightArgs a) {
   typedef typename Acc<T>::type A;
-  constexpr int VEC = VecOf<T>::value, U = PER_LANE / VEC, LANES = WAVES * 64;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int team = wave / WAVES, at = threadIdx.x - team * LANES;
+  constexpr int VEC = VecOf<T>::value, U = PER_LANE / VEC, SPAN = 64 * VEC;
+  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t b = blockIdx.y;
-  __shared__ A red[2][2][WAVES];
   A acc[PER_LANE];
 #pragma unroll
   for (int e = 0; e < PER_LANE; ++e) acc[e] = (A)0;
-  int flip = 0;
-  for (int64_t r = (int64_t)blockIdx.x * NTEAMS + team; r < a.sc.R; r += (int64_t)a.groups * NTEAMS) {
+  for (int64_t r = (int64_t)blockIdx.x * TEAMS + team; r < a.sc.R; r += (int64_t)a.groups * TEAMS) {
     const A u = a.row_weights ? static_cast<const A*>(a.row_weights)[b * a.sc.R + r] : (A)1;
-    if (u == (A)0) continue; // uniform over the team
+    if (u == (A)0) continue; // uniform
     const A c = temperature_scale(row_temperature<A>(a.sc, b, r));
     const Row<T> v = row_view<T>(a.sc, b, r);
     A x[PER_LANE];
-    load_step<T, VEC, U>(v, 0, LANES * VEC, at * VEC, x);
-    const int live = (v.n + LANES * VEC - 1) / (LANES * VEC); // vectors of the lanes that the row reaches into
+    load_step<T, VEC, U>(v, 0, SPAN, lane * VEC, x);
+    const int live = (v.n + SPAN - 1) / (SPAN); // vectors of the lanes that the row reaches into
     A m = x[0];
 #pragma unroll
     for (int e = 1; e < PER_LANE; ++e) m = fmax(m, x[e]);
     m = wave_max(m);
-    if (WAVES > 1) { // two buffers: a row's values are overwritten two barriers after they were read
-      if ((threadIdx.x & 63) == 0) red[flip][0][wave] = m;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) m = fmax(m, red[flip][0][w]);
-    }
     const A ref = finite_max(m);
     A s = (A)0;
 #pragma unroll
@@ -91,18 +84,10 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
       }
     }
     s = wave_sum(s);
-    if (WAVES > 1) {
-      if ((threadIdx.x & 63) == 0) red[flip][1][wave] = s;
-      __syncthreads();
-      s = (A)0;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) s += red[flip][1][w];
-      flip ^= 1;
-    }
     if (s == (A)0) continue; // nothing in this row may be chosen
     const A f = u / s;
     if (f != f) { // NaN for what may be chosen, nothing for what may not
-      load_step<T, VEC, U>(v, 0, LANES * VEC, at * VEC, x);
+      load_step<T, VEC, U>(v, 0, SPAN, lane * VEC, x);
 #pragma unroll
       for (int e = 0; e < PER_LANE; ++e) acc[e] += x[e] == neg_inf<A>() ? (A)0 : f;
     } else {
@@ -114,28 +99,143 @@ __global__ __launch_bounds__(WAVES* NTEAMS * 64) void pool_weights_kernel(Weight
       }
     }
   }
-  if (NTEAMS > 1) { // the teams' sums in the order of the teams, into the first one's registers
-    __shared__ A sum[LANES * PER_LANE];
-    for (int t = NTEAMS - 1; t > 0; --t) {
-      if (team == t) {
+  // the waves' sums in their order, into the first one's registers
+  __shared__ A sum[64 * PER_LANE];
+  for (int t = TEAMS - 1; t > 0; --t) {
+    if (team == t) {
 #pragma unroll
-        for (int e = 0; e < PER_LANE; ++e) sum[e * LANES + at] = (t == NTEAMS - 1 ? (A)0 : sum[e * LANES + at]) + acc[e];
-      }
-      __syncthreads();
+      for (int e = 0; e < PER_LANE; ++e) sum[e * 64 + lane] = (t == TEAMS - 1 ? (A)0 : sum[e * 64 + lane]) + acc[e];
     }
-    if (team != 0) return;
+    __syncthreads();
+  }
+  if (team != 0) return;
 #pragma unroll
-    for (int e = 0; e < PER_LANE; ++e) acc[e] += sum[e * LANES + at];
+  for (int e = 0; e < PER_LANE; ++e) acc[e] += sum[e * 64 + lane];
+#pragma unroll
+  for (int w = 0; w < U; ++w) store_sums<A, VEC>(a, b, blockIdx.x, 0, w * SPAN + lane * VEC, acc + w * VEC);
+}
+
+// One pass over longer pools: a row a workgroup of WAVES waves, which meet at a barrier for the largest score and at one for the
+// sum.  What is needed of the rows (scale, weight, length) is fetched for 64 at a time, and the next row's scores are on their
+// way while one is worked on (DENSE: candidates, and mask bytes, side by side; else they are loaded where they are used).
+// One workgroup of 16 waves fills a CU's registers, so a row's two barriers and reductions stand in the open: 2048 x 16384
+// float32 take 32.7 us (4.1 TB/s; the vector units are busy half of it, 20 instructions a score), 16 x 128 x 16381 35 us, with
+// rows half as long on average 32, and 6 to join.  The two passes of longer pools would take 51 and 52.  4 waves up to 4096
+// candidates: 2000 x 4096 float32 12.6 us and 8.6 to join, with 16 waves 21.5 and 4.6; float64 1000 x 4096 17.3 against 19.6.
+constexpr int ROW_BLOCK = 64;
+template <typename A>
+struct WorkRow {
+  A c, u;
+  int n;
+};
+template <typename T, int WAVES, bool DENSE>
+__global__ __launch_bounds__(WAVES * 64) void pool_weights_kernel(WeightArgs a) {
+  typedef typename Acc<T>::type A;
+  constexpr int VEC = VecOf<T>::value, U = PER_LANE / VEC, LANES = WAVES * 64, SPAN = LANES * VEC;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = threadIdx.x, M = a.sc.M;
+  const int64_t b = blockIdx.y;
+  __shared__ WorkRow<A> rows[ROW_BLOCK];
+  __shared__ A red[2][WAVES]; // each half is read before the barrier of the other one, and written after it
+  A acc[PER_LANE];
+#pragma unroll
+  for (int e = 0; e < PER_LANE; ++e) acc[e] = (A)0;
+  const int64_t stride = a.groups;
+  RawStep<T, VEC, U, DENSE> raw;
+  const T* x0 = static_cast<const T*>(a.sc.x) + b * a.sc.xb;
+  const uint8_t* mask0 = a.sc.mask ? a.sc.mask + b * a.sc.mb : nullptr;
+#pragma unroll 1
+  for (int64_t r0 = blockIdx.x; r0 < a.sc.R; r0 += stride * ROW_BLOCK) {
+    const int64_t left = (a.sc.R - r0 + stride - 1) / stride;
+    const int count = left < ROW_BLOCK ? (int)left : ROW_BLOCK;
+    __syncthreads();
+    if (at < count) {
+      const int64_t r = r0 + at * stride;
+      WorkRow<A> k;
+      k.u = a.row_weights ? static_cast<const A*>(a.row_weights)[b * a.sc.R + r] : (A)1;
+      k.c = temperature_scale(row_temperature<A>(a.sc, b, r));
+      k.n = k.u == (A)0 ? 0 : row_length(a.sc, b, r);
+      rows[at] = k;
+    }
+    __syncthreads();
+    auto row = [&](int q) {
+      WorkRow<A> k = rows[q];
+      k.n = __builtin_amdgcn_readfirstlane(k.n);
+      return k;
+    };
+    auto view = [&](int q, int n) {
+      const int64_t r = r0 + q * stride;
+      return Row<T>{x0 + r * a.sc.xr, mask0 ? mask0 + r * a.sc.mr : nullptr, a.sc.xc, a.sc.mc, n};
+    };
+    WorkRow<A> next = row(0);
+    if (DENSE) raw.load(view(0, next.n), M, SPAN, at * VEC);
+#pragma unroll 1
+    for (int q = 0; q < count; ++q) {
+      const WorkRow<A> k = next;
+      A x[PER_LANE];
+      if (DENSE) raw.decode(mask0 != nullptr, k.n, M, SPAN, at * VEC, x);
+      if (q + 1 < count) {
+        next = row(q + 1);
+        if (DENSE) raw.load(view(q + 1, next.n), M, SPAN, at * VEC);
+      }
+      if (k.n == 0) continue;
+      if (!DENSE) load_step<T, VEC, U>(view(q, k.n), 0, SPAN, at * VEC, x);
+      const A c = k.c, u = k.u;
+      const int n = k.n;
+      A m = x[0];
+#pragma unroll
+      for (int e = 1; e < PER_LANE; ++e) m = fmax(m, x[e]);
+      m = wave_max(m);
+      if ((threadIdx.x & 63) == 0) red[0][wave] = m;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) m = fmax(m, red[0][w]);
+      const A ref = finite_max(m);
+      A s = (A)0;
+      uint32_t there = 0; // which of this lane's candidates exist, for a row that is NaN
+#pragma unroll
+      for (int w = 0; w < U; ++w) {
+        if (w * SPAN >= n) break; // uniform
+#pragma unroll
+        for (int e = w * VEC; e < (w + 1) * VEC; ++e) {
+          there |= (uint32_t)(x[e] != neg_inf<A>()) << e;
+          x[e] = exp2_acc((x[e] - ref) * c);
+          s += x[e];
+        }
+      }
+      s = wave_sum(s);
+      if ((threadIdx.x & 63) == 0) red[1][wave] = s;
+      __syncthreads();
+      s = (A)0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) s += red[1][w];
+      if (s == (A)0) continue; // nothing in this row may be chosen
+      const A f = u / s;
+      if (f != f) { // NaN for what may be chosen, nothing for what may not
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e) acc[e] += (there >> e) & 1 ? f : (A)0;
+      } else {
+#pragma unroll
+        for (int w = 0; w < U; ++w) {
+          if (w * SPAN >= n) break;
+#pragma unroll
+          for (int e = w * VEC; e < (w + 1) * VEC; ++e) acc[e] = fma(x[e], f, acc[e]);
+        }
+      }
+    }
   }
 #pragma unroll
-  for (int w = 0; w < U; ++w) store_sums<A, VEC>(a, b, blockIdx.x, 0, w * LANES * VEC + at * VEC, acc + w * VEC);
+  for (int w = 0; w < U; ++w) {
+    const int j = w * SPAN + at * VEC;
+    store_sums<A, VEC>(a, b, blockIdx.x, j, DENSE && j > M - VEC ? M - VEC : j, acc + w * VEC);
+  }
 }
 
 // Second pass over longer pools: a workgroup sums a tile of 256 lanes' vectors over its share of rows.  What it needs of a row
 // (scale, reference, log of the sum, weight, length) it joins itself from the first pass's partial results, 64 rows at a time in
 // LDS; the next row that reaches into the tile is on its way while one is worked on; a mask that all rows share is read once.
 // A vector that would cross the end of the pool starts earlier, and only its own candidates are written.  DENSE: candidates (and
-// mask bytes) side by side.
+// mask bytes) side by side.  64 x 262144 float64 with a shared mask: 36 us (3.7 TB/s, behind 28 us of the first pass), float32
+// 15.2 us (4.4 TB/s), bfloat16 16.4: exponentials and 64-bit arithmetic, then memory.
 constexpr int COL_BLOCK = 64;
 constexpr int col_vecs(int size) { return size == 2 ? 1 : 2; } // vectors a lane holds of a row (one is 8 scores of 16 bits)
 template <typename A>
@@ -236,7 +336,8 @@ __global__ __launch_bounds__(256) void pool_columns_kernel(WeightArgs a) {
   for (int u = 0; u < U; ++u) store_sums<A, VEC>(a, b, blockIdx.y, j0 + u * SPAN + (int)threadIdx.x * VEC, off[u], acc + u * VEC);
 }
 
-// decay w + the groups' partial sums in their order: 64 candidates per workgroup, the groups dealt to its four waves
+// decay w + the groups' partial sums in their order: 64 candidates per workgroup, the groups dealt to its four waves.  4 to 9 us,
+// most of it the launch (16 x 16 groups x 16381: 17 MB, 6 us).
 template <typename A>
 __global__ __launch_bounds__(256) void pool_weights_join_kernel(WeightArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -271,7 +372,9 @@ __global__ __launch_bounds__(256) void pool_weights_join_kernel(WeightArgs a) {
 // the launches.
 
 constexpr int EVICT_PAYLOADS = 16;
-constexpr int FUSED_ROW_BYTES = 64; // payload rows up to this are moved by the lane that keeps the candidate
+// Payload rows up to this are moved by the lane that keeps the candidate, longer ones by a launch of their own: of 64 pools of
+// 16384, cut to 4096, rows of 24 bytes take 26.6 us in all against 20.9 + 4.5, of 64 bytes 36.9 against 22.0 + 7.9.
+constexpr int FUSED_ROW_BYTES = 32;
 
 struct Payload {
   const char* src;
@@ -538,7 +641,9 @@ __device__ __forceinline__ void put_marked(const EvictArgs& a, int64_t b, int64_
   put_kept<W>(a, b, base, j0, kept, total);
 }
 
-// One workgroup per pool of at most 1024 PER candidates.
+// One workgroup per pool of at most 1024 PER candidates, whose keys stay in its registers: a chain of barriers (range, two or three
+// histograms of 12 bits, places), 9 us for 1000 candidates, 12 for 4096, 22 for 16384, 27 for 64 pools of that.  Over five
+// launches 16384 take 29 us and the gaps between them, 64 pools of that 33.
 template <typename W, int PER>
 __global__ __launch_bounds__(1024) void pool_evict_kernel(EvictArgs a) {
   typedef typename KeyOf<W>::type Key;
@@ -911,6 +1016,7 @@ __global__ __launch_bounds__(1024) void pool_evict_put_kernel(EvictArgs a) {
 }
 
 // Payload rows too long for that, of one pool a grid row: 2^log_lanes lanes a row, moved in units; zeros where nothing stayed.
+// 64 x 4096 rows of 256 bytes: 20 us (134 MB read and written, 6.6 TB/s); one pool's 4096 rows of 64 bytes: the launch, 4 us.
 template <typename Unit>
 __global__ __launch_bounds__(256) void pool_gather_kernel(const int64_t* indices, const Unit* src, Unit* dst, int64_t K, int64_t M, int units, int log_lanes) {
   const int64_t b = blockIdx.y;
@@ -932,7 +1038,7 @@ void gather_launch(const int64_t* indices, const void* src, void* dst, int64_t p
                      static_cast<const Unit*>(src), static_cast<Unit*>(dst), K, M, (int)units, log_lanes);
 }
 
-// Teams that work off a pool's rows in the one-pass kernel, and groups (workgroups) of them.
+// Waves a row in the one-pass kernels, and groups (workgroups); the kernels' comments have both sides of each rule.
 struct WeightPlan {
   bool one_pass;
   int waves, groups;
@@ -979,12 +1085,18 @@ void weights_launch(const WeightArgs& a, const WeightPlan& p, int64_t pools, hip
   typedef typename Acc<T>::type A;
   if (p.one_pass) {
     const dim3 grid(a.groups, (unsigned)pools);
+    const bool dense = a.sc.xc == 1 && (!a.sc.mask || a.sc.mc == 1);
+    constexpr int MOST = sizeof(T) == 8 ? 8 : 16;
     if (p.waves == 1)
-      hipLaunchKernelGGL((pool_weights_kernel<T, 1, TEAMS>), grid, dim3(TEAMS * 64), 0, st, a);
+      hipLaunchKernelGGL(pool_weights_wave_kernel<T>, grid, dim3(TEAMS * 64), 0, st, a);
+    else if (p.waves == 4 && dense)
+      hipLaunchKernelGGL((pool_weights_kernel<T, 4, true>), grid, dim3(256), 0, st, a);
     else if (p.waves == 4)
-      hipLaunchKernelGGL((pool_weights_kernel<T, 4, 1>), grid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((pool_weights_kernel<T, 4, false>), grid, dim3(256), 0, st, a);
+    else if (dense)
+      hipLaunchKernelGGL((pool_weights_kernel<T, MOST, true>), grid, dim3(MOST * 64), 0, st, a);
     else
-      hipLaunchKernelGGL((pool_weights_kernel<T, sizeof(T) == 8 ? 8 : 16, 1>), grid, dim3(p.waves * 64), 0, st, a);
+      hipLaunchKernelGGL((pool_weights_kernel<T, MOST, false>), grid, dim3(MOST * 64), 0, st, a);
   } else {
     const int tile = 256 * VecOf<T>::value * col_vecs(sizeof(T));
     const unsigned tiles = (unsigned)((a.sc.M + tile - 1) / tile);
@@ -1002,7 +1114,7 @@ int payload_unit(const void* src, const void* dst, int64_t row_bytes) {
   const uintptr_t al = (uintptr_t)src | (uintptr_t)dst | (uintptr_t)row_bytes;
   return al % 16 == 0 ? 16 : al % 8 == 0 ? 8 : al % 4 == 0 ? 4 : al % 2 == 0 ? 2 : 1;
 }
-constexpr int64_t HELD_MAX = 16 * 1024; // candidates that one workgroup holds in its registers
+constexpr int64_t HELD_MAX = 16 * 1024; // candidates that one workgroup holds in its registers (both sides: pool_evict_kernel)
 int64_t evict_workspace(int dtype, int64_t pools, int64_t M) {
   if (M <= HELD_MAX) return 0;
   const int64_t chunks = (M + CHUNK - 1) / CHUNK;
