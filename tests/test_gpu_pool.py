@@ -555,3 +555,40 @@ def test_alternatives_of_scores_that_lie_close_together(kind, shape, sign):
         for top in (1, 20, 25, 64):
             r = acq.choice_logprobs(x, top=top)
             np.testing.assert_array_equal(host(r.top_indices), ref.choice(host(x), top=top)["top_indices"])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("shape", [(600, 133, 1030), (300, 140, 4500), (260, 135, 9001), (1, 9001, 16500)], ids=str)
+def test_pool_weights_of_many_rows(kind, shape):
+    """More rows than a workgroup fetches the particulars of at once, in both kernels; some of them empty, of weight 0 or NaN."""
+    g = torch.Generator(device="cuda").manual_seed(shape[1])
+    pools, R, M = shape
+    x = torch.empty(shape, device="cuda", dtype=getattr(torch, kind)).normal_(generator=g).mul_(2)
+    lengths = torch.randint(0, M + 1, (pools, R), device="cuda", generator=g)
+    lengths[:, ::7] = 0
+    lengths[:, 1::7] = M
+    u = torch.rand(pools, R, device="cuda", generator=g, dtype=ACC[kind])
+    u[:, 3::5] = 0
+    mask = torch.rand(M, device="cuda", generator=g) > 0.2
+    x[:, 70, :3] = math.nan
+    u[: (pools + 1) // 2, 70] = 0  # half of the pools do not read it
+    got = acq.pool_weights(x, row_weights=u, temperature=0.7, mask=mask, lengths=lengths)
+    want = torch.zeros(pools, M, device="cuda", dtype=torch.float64)
+    at = torch.arange(M, device="cuda")
+    poisoned = torch.zeros(pools, M, dtype=torch.bool, device="cuda")
+    for r0 in range(0, R, 128):
+        z = x[:, r0:r0 + 128].double() / 0.7
+        ok = mask & (at < lengths[:, r0:r0 + 128, None])
+        if r0 <= 70 < r0 + 128:
+            n, v = ok[:, 70 - r0], u[:, 70]
+            poisoned = n & ((v != 0) & (n & torch.isnan(x[:, 70])).any(1))[:, None]
+            z[:, 70 - r0] = 0
+            ok[:, 70 - r0] = False
+        z.masked_fill_(~ok, -math.inf)
+        e = torch.exp(z - z.amax(2, keepdim=True).clamp_min(-1e300))  # (torch.softmax of float64 is right to 1e-7 only here)
+        p = e / e.sum(2, keepdim=True).clamp_min(1e-300)
+        want += torch.bmm(u[:, None, r0:r0 + 128].double(), p.contiguous())[:, 0]
+    want[poisoned] = math.nan
+    tol = ref.U[kind] * (200 + M / 64 + 8 * 120 + 8 + R) * (host(want.nan_to_num(0.0)) + 2 ** -1000)
+    close(host(got), host(want), tol, "weights")
+    assert torch.equal(got[: (pools + 1) // 2].nan_to_num(7), acq.pool_weights(x, row_weights=u, temperature=0.7, mask=mask, lengths=lengths)[: (pools + 1) // 2].nan_to_num(7))
