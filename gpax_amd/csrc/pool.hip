@@ -367,9 +367,9 @@ __global__ __launch_bounds__(256) void pool_weights_join_kernel(WeightArgs a) {
 // prefix stay, of those equal to it the first in order.  Counts only: no result depends on the order of an atomic.
 //
 // One workgroup per pool where the pool fits its registers (16384 candidates).  Longer pools are cut into chunks of 4096, a
-// workgroup each, over five launches: range of the keys | histogram of 12 bits | of the next 12 | the few candidates that
-// share all 24 (or that need no telling apart) | output.  Read five times, but 2 MB of weights stay in the caches: bound by
-// the launches.
+// workgroup each, over six launches: range of the keys | histograms of 12, 12 and 12 bits | the few candidates that share all
+// 36 (or that need no telling apart) | output.  Read six times, but 2 MB of weights stay in the caches: bound by the launches.
+// 64-bit weights of more than THREE_DIGITS_MAX candidates have a histogram for every 12 bits of a key.
 
 constexpr int EVICT_PAYLOADS = 16;
 // Payload rows up to this are moved by the lane that keeps the candidate, longer ones by a launch of their own: of 64 pools of
@@ -393,6 +393,7 @@ struct EvictArgs {
   int npay;
   void* ws;
   int64_t chunks;
+  int levels; // histograms
   Payload pay[EVICT_PAYLOADS];
 };
 
@@ -642,8 +643,8 @@ __device__ __forceinline__ void put_marked(const EvictArgs& a, int64_t b, int64_
 }
 
 // One workgroup per pool of at most 1024 PER candidates, whose keys stay in its registers: a chain of barriers (range, two or three
-// histograms of 12 bits, places), 9 us for 1000 candidates, 12 for 4096, 22 for 16384, 27 for 64 pools of that.  Over five
-// launches 16384 take 29 us and the gaps between them, 64 pools of that 33.
+// histograms of 12 bits, places), 9 us for 1000 candidates, 12 for 4096, 22 for 16384, 27 for 64 pools of that.  Over six
+// launches 16384 take 32 us and the gaps between them, 64 pools of that 38.
 template <typename W, int PER>
 __global__ __launch_bounds__(1024) void pool_evict_kernel(EvictArgs a) {
   typedef typename KeyOf<W>::type Key;
@@ -705,16 +706,23 @@ __global__ __launch_bounds__(1024) void pool_evict_kernel(EvictArgs a) {
   if (tid == 0) a.new_lengths[b] = cut.keep;
 }
 
-// ---- longer pools: chunks of 4096, five launches ----
+// ---- longer pools: chunks of 4096, six launches and more ----
 constexpr int CHUNK_PER = 4, CHUNK = 1024 * CHUNK_PER;
 constexpr int MAX_TIED = 1024; // candidates told apart one by one in the last launch
+// Three digits are all of a 32-bit key.  Of a 64-bit one they leave those that agree in 36 bits, counted from the highest that
+// differs, to the last launch; if those are many, each workgroup goes through the whole pool, 0.4 ms at 262144 candidates and 1.3
+// at this size, growing with the square.  (After two digits that already happens to weights within 2^-14 of each other beside
+// one that is larger; the third launch costs 3 us.)  Beyond it a launch for every digit that a key has.
+constexpr int64_t THREE_DIGITS_MAX = 1 << 19;
+template <typename Key>
+constexpr int DIGITS = (8 * (int)sizeof(Key) + WIDE_BITS - 1) / WIDE_BITS;
 
 template <typename Key>
 struct EvictState { // per pool; behind it, per chunk: {all, any} of Key, counts above and at the prefix
-  uint32_t hist[2][WIDE_BINS];
-  Key prefix[3];    // after the range, the first and the second histogram
-  int shift[3];
-  uint32_t need[3], count[3]; // still needed of those at the prefix; how many there are
+  uint32_t hist[DIGITS<Key>][WIDE_BINS];
+  Key prefix[DIGITS<Key> + 1]; // after the range and after each histogram
+  int shift[DIGITS<Key> + 1];
+  uint32_t need[DIGITS<Key> + 1], count[DIGITS<Key> + 1]; // still needed of those at the prefix; how many there are
   uint32_t tied;    // candidates collected
   Key tied_key[MAX_TIED];
   uint32_t tied_idx[MAX_TIED];
@@ -762,7 +770,7 @@ __global__ __launch_bounds__(1024) void pool_evict_range_kernel(EvictArgs a) {
   const int64_t b = blockIdx.y, c = blockIdx.x;
   const PoolCut cut = pool_cut(a, b);
   const EvictView<Key> v = evict_view<Key>(a, b);
-  for (int64_t i = c * 1024 + threadIdx.x; i < 2 * WIDE_BINS; i += a.chunks * 1024) (&v.st->hist[0][0])[i] = 0;
+  for (int64_t i = c * 1024 + threadIdx.x; i < a.levels * WIDE_BINS; i += a.chunks * 1024) (&v.st->hist[0][0])[i] = 0;
   if (c == 0 && threadIdx.x == 0) v.st->tied = 0;
   Chunk<W> k;
   k.load(a, cut, b, c * CHUNK);
@@ -782,18 +790,18 @@ __global__ __launch_bounds__(1024) void pool_evict_range_kernel(EvictArgs a) {
   }
 }
 
-// What is known of a pool's prefix before launch LEVEL (1, 2: a histogram; 3: collecting): from the launch before, and written
-// for the next by the first chunk.  Nothing is left to decide where need == 0 or every candidate at the prefix stays.
+// What is known of a pool's prefix before launch `level` (1, 2 ...: a histogram; behind them: collecting): from the launch
+// before, and written for the next by the first chunk.  Nothing is left to decide where need == 0 or every candidate at the prefix stays.
 template <typename Key>
 struct Prefix {
   Key prefix;
   int shift;
   uint32_t need, count;
 };
-template <typename Key, int LEVEL>
-__device__ __forceinline__ Prefix<Key> advance_prefix(const EvictArgs& a, const EvictView<Key>& v, const PoolCut& cut, Key (*sh_keys)[16]) {
+template <typename Key, bool FIRST>
+__device__ __forceinline__ Prefix<Key> advance_prefix(const EvictArgs& a, const EvictView<Key>& v, const PoolCut& cut, int level, Key (*sh_keys)[16]) {
   Prefix<Key> p;
-  if (LEVEL == 1) {
+  if (FIRST) {
     Key all = ~(Key)0, any = 0;
     for (int64_t i = threadIdx.x; i < a.chunks; i += 1024) {
       all &= v.ch[i].all;
@@ -806,10 +814,10 @@ __device__ __forceinline__ Prefix<Key> advance_prefix(const EvictArgs& a, const 
     p.need = cut.need;
     p.count = (uint32_t)(cut.hi - cut.lo);
   } else {
-    p = Prefix<Key>{v.st->prefix[LEVEL - 2], v.st->shift[LEVEL - 2], v.st->need[LEVEL - 2], v.st->count[LEVEL - 2]};
+    p = Prefix<Key>{v.st->prefix[level - 2], v.st->shift[level - 2], v.st->need[level - 2], v.st->count[level - 2]};
     if (p.shift > 0 && p.need > 0 && p.need < p.count) {
       const int lo = p.shift > WIDE_BITS ? p.shift - WIDE_BITS : 0, width = p.shift - lo;
-      const Digit d = wide_digit(v.st->hist[LEVEL - 2], p.need);
+      const Digit d = wide_digit(v.st->hist[level - 2], p.need);
       p.prefix = (p.prefix << width) | (Key)d.bin;
       p.shift = lo;
       p.need -= d.above;
@@ -817,16 +825,16 @@ __device__ __forceinline__ Prefix<Key> advance_prefix(const EvictArgs& a, const 
     }
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    v.st->prefix[LEVEL - 1] = p.prefix;
-    v.st->shift[LEVEL - 1] = p.shift;
-    v.st->need[LEVEL - 1] = p.need;
-    v.st->count[LEVEL - 1] = p.count;
+    v.st->prefix[level - 1] = p.prefix;
+    v.st->shift[level - 1] = p.shift;
+    v.st->need[level - 1] = p.need;
+    v.st->count[level - 1] = p.count;
   }
   return p;
 }
 
-template <typename W, int LEVEL>
-__global__ __launch_bounds__(1024) void pool_evict_hist_kernel(EvictArgs a) {
+template <typename W, bool FIRST>
+__global__ __launch_bounds__(1024) void pool_evict_hist_kernel(EvictArgs a, int level) {
   typedef typename KeyOf<W>::type Key;
   __shared__ uint32_t bins[WIDE_BINS];
   __shared__ Key sh_keys[2][16];
@@ -835,7 +843,7 @@ __global__ __launch_bounds__(1024) void pool_evict_hist_kernel(EvictArgs a) {
   const EvictView<Key> v = evict_view<Key>(a, b);
   Chunk<W> k;
   k.load(a, cut, b, c * CHUNK);
-  const Prefix<Key> p = advance_prefix<Key, LEVEL>(a, v, cut, sh_keys);
+  const Prefix<Key> p = advance_prefix<Key, FIRST>(a, v, cut, level, sh_keys);
   if (p.shift == 0 || p.need == 0 || p.need == p.count) return;
   __syncthreads();
   for (int i = threadIdx.x; i < WIDE_BINS; i += 1024) bins[i] = 0;
@@ -846,7 +854,7 @@ __global__ __launch_bounds__(1024) void pool_evict_hist_kernel(EvictArgs a) {
     if (((k.free_bits >> i) & 1) && above(k.key[i], p.shift) == p.prefix) atomicAdd(&bins[(uint32_t)(k.key[i] >> lo) & ((1u << width) - 1u)], 1u);
   __syncthreads();
   for (int i = threadIdx.x; i < WIDE_BINS; i += 1024)
-    if (bins[i]) atomicAdd(&v.st->hist[LEVEL - 1][i], bins[i]);
+    if (bins[i]) atomicAdd(&v.st->hist[level - 1][i], bins[i]);
 }
 
 template <typename W>
@@ -859,7 +867,7 @@ __global__ __launch_bounds__(1024) void pool_evict_collect_kernel(EvictArgs a) {
   const EvictView<Key> v = evict_view<Key>(a, b);
   Chunk<W> k;
   k.load(a, cut, b, c * CHUNK);
-  const Prefix<Key> p = advance_prefix<Key, 3>(a, v, cut, sh_keys);
+  const Prefix<Key> p = advance_prefix<Key, false>(a, v, cut, a.levels + 1, sh_keys);
   const bool open = p.shift > 0 && p.need > 0 && p.need < p.count;
   uint32_t g = 0, e = 0;
   Key all = ~(Key)0, any = 0;
@@ -873,12 +881,22 @@ __global__ __launch_bounds__(1024) void pool_evict_collect_kernel(EvictArgs a) {
       e += 1;
       all &= k.key[i];
       any |= k.key[i];
-      if (open && p.count <= MAX_TIED) { // in no particular order: the last launch ranks them
-        const uint32_t at = atomicAdd(&v.st->tied, 1u);
-        v.st->tied_key[at] = k.key[i];
-        v.st->tied_idx[at] = (uint32_t)j;
-      }
     }
+  }
+  if (open && p.count <= MAX_TIED) { // uniform; in no particular order, which decides nothing
+    __shared__ uint32_t found, base;
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    uint32_t at = e > 0 ? atomicAdd(&found, e) : 0;
+    __syncthreads();
+    if (threadIdx.x == 0) base = found > 0 ? atomicAdd(&v.st->tied, found) : 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < CHUNK_PER; ++i)
+      if (((k.free_bits >> i) & 1) && above(k.key[i], p.shift) == p.prefix) {
+        v.st->tied_key[base + at] = k.key[i];
+        v.st->tied_idx[base + at++] = (uint32_t)(c * CHUNK + i * 1024 + threadIdx.x);
+      }
   }
   g = wave_sum(g);
   e = wave_sum(e);
@@ -904,17 +922,14 @@ __global__ __launch_bounds__(1024) void pool_evict_collect_kernel(EvictArgs a) {
 template <typename W>
 __global__ __launch_bounds__(1024) void pool_evict_put_kernel(EvictArgs a) {
   typedef typename KeyOf<W>::type Key;
-  __shared__ Key sh_key[MAX_TIED];
-  __shared__ uint32_t sh_idx[MAX_TIED], bins[WIDE_BINS];
+  __shared__ uint32_t bins[WIDE_BINS];
   __shared__ Key sh_keys[2][16];
   __shared__ uint32_t sh_sum[4][16];
-  __shared__ Key cut_key;
-  __shared__ uint32_t cut_idx;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t b = blockIdx.y, c = blockIdx.x, j0 = c * CHUNK;
   const PoolCut cut = pool_cut(a, b);
   const EvictView<Key> v = evict_view<Key>(a, b);
-  Prefix<Key> p{v.st->prefix[2], v.st->shift[2], v.st->need[2], v.st->count[2]};
+  Prefix<Key> p{v.st->prefix[a.levels], v.st->shift[a.levels], v.st->need[a.levels], v.st->count[a.levels]};
   Chunk<W> k;
   k.load(a, cut, b, j0);
   // candidates before this chunk that stay, or are at the prefix; whether all at the prefix are the same
@@ -934,35 +949,50 @@ __global__ __launch_bounds__(1024) void pool_evict_put_kernel(EvictArgs a) {
   all = block_reduce(all, sh_keys[0], key_and<Key>);
   any = block_reduce(any, sh_keys[1], key_or<Key>);
   bool open = p.shift > 0 && p.need > 0 && p.need < p.count;
-  bool by_place = false; // ties are cut at (cut_key, cut_idx) instead of by their number
+  bool by_place = false; // ties are cut by their keys and places instead of by their number
   if (open && all == any) {
     p.shift = 0; // the first `need` of equal weights
     p.prefix = all;
     open = false;
   }
-  if (open && p.count <= MAX_TIED) {
-    if (tid < (int)p.count) {
-      sh_key[tid] = v.st->tied_key[tid];
-      sh_idx[tid] = v.st->tied_idx[tid];
-    }
-    __syncthreads();
-    uint32_t taken_before = 0;
-    if (tid < (int)p.count) {
-      const Key kk = sh_key[tid];
-      const uint32_t ii = sh_idx[tid];
-      uint32_t rank = 0;
-      for (uint32_t q = 0; q < p.count; ++q) rank += sh_key[q] > kk || (sh_key[q] == kk && sh_idx[q] < ii);
-      if (rank == p.need - 1) {
-        cut_key = kk;
-        cut_idx = ii;
+  Key tie_prefix = 0;
+  uint32_t place_prefix = 0;
+  int tie_shift = 0, place_shift = 32;
+  if (open && p.count <= MAX_TIED) { // a candidate a thread: the other digits of their keys, then those of their places
+    const bool in = tid < (int)p.count;
+    const Key kk = in ? v.st->tied_key[tid] : (Key)0;
+    const uint32_t place = in ? ~v.st->tied_idx[tid] : 0; // the lower, the better
+    uint32_t n = p.need, left = p.count;
+    tie_prefix = p.prefix;
+    tie_shift = p.shift;
+    while (n < left && (tie_shift > 0 || place_shift > 0)) {
+      const bool by_key = tie_shift > 0;
+      const int from = by_key ? tie_shift : place_shift, lo = from > WIDE_BITS ? from - WIDE_BITS : 0, width = from - lo;
+      __syncthreads();
+      for (int i = tid; i < WIDE_BINS; i += 1024) bins[i] = 0;
+      __syncthreads();
+      if (in && above(kk, tie_shift) == tie_prefix && above(place, place_shift) == place_prefix)
+        atomicAdd(&bins[(by_key ? (uint32_t)(kk >> lo) : place >> lo) & ((1u << width) - 1u)], 1u);
+      __syncthreads();
+      const Digit d = wide_digit(bins, n);
+      if (by_key) {
+        tie_prefix = (tie_prefix << width) | (Key)d.bin;
+        tie_shift = lo;
+      } else {
+        place_prefix = (place_prefix << width) | (uint32_t)d.bin;
+        place_shift = lo;
       }
-      taken_before = rank < p.need && (int64_t)ii < j0;
+      n -= d.above;
+      left = d.count;
     }
+    const Key hi = above(kk, tie_shift);
+    const bool taken = in && (hi > tie_prefix || (hi == tie_prefix && above(place, place_shift) >= place_prefix));
+    const uint32_t taken_before = taken && (int64_t)(uint32_t)~place < j0;
     e0 = block_reduce(taken_before, sh_sum[2], add);
     by_place = true;
   } else if (open) {
-    // many candidates that agree in 24 bits and differ below: this workgroup goes through the whole pool, 12 bits at a time,
-    // and counts what lies before its chunk.  Slow, and rare: weights closer than one part in 4096 all over the pool
+    // many candidates that agree in 36 bits and differ below: this workgroup goes through the whole pool, 12 bits at a time,
+    // and counts what lies before its chunk.  Slow, and rare: 64-bit weights closer than 2^-26 all over the pool, and one far off
     const Key group = p.prefix;
     const int group_shift = p.shift;
     while (p.shift > 0 && p.need < p.count) {
@@ -1007,7 +1037,10 @@ __global__ __launch_bounds__(1024) void pool_evict_put_kernel(EvictArgs a) {
     const Key hi = above(k.key[i], p.shift);
     g_bits |= (uint32_t)(j < cut.L && (!fr || (p.need > 0 && hi > p.prefix))) << i;
     bool e = fr && p.need > 0 && hi == p.prefix;
-    if (by_place) e = e && (k.key[i] > cut_key || (k.key[i] == cut_key && (uint32_t)j <= cut_idx));
+    if (by_place) {
+      const Key tie = above(k.key[i], tie_shift);
+      e = e && (tie > tie_prefix || (tie == tie_prefix && above(~(uint32_t)j, place_shift) >= place_prefix));
+    }
     e_bits |= (uint32_t)e << i;
   }
   put_marked<W, CHUNK_PER>(a, b, j0, g_bits, e_bits, p.need, g0, e0, lane, wave);
@@ -1135,8 +1168,8 @@ void evict_launch(const EvictArgs& a, int64_t pools, hipStream_t st) {
   }
   const dim3 grid((unsigned)a.chunks, (unsigned)pools);
   hipLaunchKernelGGL(pool_evict_range_kernel<W>, grid, block, 0, st, a);
-  hipLaunchKernelGGL((pool_evict_hist_kernel<W, 1>), grid, block, 0, st, a);
-  hipLaunchKernelGGL((pool_evict_hist_kernel<W, 2>), grid, block, 0, st, a);
+  hipLaunchKernelGGL((pool_evict_hist_kernel<W, true>), grid, block, 0, st, a, 1);
+  for (int level = 2; level <= a.levels; ++level) hipLaunchKernelGGL((pool_evict_hist_kernel<W, false>), grid, block, 0, st, a, level);
   hipLaunchKernelGGL(pool_evict_collect_kernel<W>, grid, block, 0, st, a);
   hipLaunchKernelGGL(pool_evict_put_kernel<W>, grid, block, 0, st, a);
 }
@@ -1224,6 +1257,7 @@ int gpx_pool_evict(gpx_ctx* ctx, int dtype, int64_t pools, int64_t candidates, c
   a.out = d_weights_out;
   a.ws = d_workspace;
   a.chunks = (candidates + CHUNK - 1) / CHUNK;
+  a.levels = dtype == GPX_DTYPE_F64 && candidates > THREE_DIGITS_MAX ? DIGITS<uint64_t> : DIGITS<uint32_t>;
   for (int i = 0; i < npayload; ++i) {
     const int64_t rb = payload_row_bytes[i];
     if (rb == 0 || rb > FUSED_ROW_BYTES) continue;

@@ -592,3 +592,36 @@ def test_pool_weights_of_many_rows(kind, shape):
     tol = ref.U[kind] * (200 + M / 64 + 8 * 120 + 8 + R) * (host(want.nan_to_num(0.0)) + 2 ** -1000)
     close(host(got), host(want), tol, "weights")
     assert torch.equal(got[: (pools + 1) // 2].nan_to_num(7), acq.pool_weights(x, row_weights=u, temperature=0.7, mask=mask, lengths=lengths)[: (pools + 1) // 2].nan_to_num(7))
+
+
+@pytest.mark.parametrize("kind", ["float64", "float32"])
+@pytest.mark.parametrize("shape", [(65536,), (524288,), (524289,), (2, 700001), (3, 1048577)], ids=str)
+def test_evict_from_very_long_pools(kind, shape):
+    """Pools of up to 2^19 candidates and more; many of them may agree in their upper bits, or in all of them."""
+    g = torch.Generator(device="cuda").manual_seed(shape[-1])
+    M, budget = shape[-1], shape[-1] // 3
+    tiny = 2.0 ** (-23 if kind == "float32" else -52)
+    uniform = torch.rand(shape, device="cuda", generator=g, dtype=torch.float64)
+    near = 1.0 + torch.randint(0, 200, shape, device="cuda", generator=g) * tiny
+    outlier = near.clone()
+    outlier[..., M // 2] = 1e30
+    flat_top = 1.0 + 1e-5 * uniform  # nothing but the last 36 bits
+    flat_top[..., 7] = 100.0
+    for values in (uniform, near, outlier, flat_top, torch.zeros_like(near), torch.exp(3 * torch.randn(shape, device="cuda", generator=g, dtype=torch.float64))):
+        w = values.to(getattr(torch, kind))
+        pts = torch.rand(shape + (2,), device="cuda", generator=g)
+        got = acq.pool_evict(w, budget, (pts,), first=3, recent=10)
+        flat = w.reshape(-1, M)
+        for b in range(len(flat)):
+            free = flat[b, 3:M - 10]
+            order = torch.sort(free, descending=True, stable=True).indices[:budget - 13] + 3
+            want = torch.cat([torch.arange(3, device="cuda"), torch.sort(order).values, torch.arange(M - 10, M, device="cuda")])
+            assert torch.equal(got.indices.reshape(-1, budget)[b], want)
+            assert torch.equal(got.payload[0].reshape(-1, budget, 2)[b], pts.reshape(-1, M, 2)[b][want])
+
+
+def test_evict_from_forty_million():
+    w = torch.rand(40_000_000, device="cuda", dtype=torch.float64)
+    got = acq.pool_evict(w, 1000)
+    want = torch.sort(torch.topk(w, 1000).indices).values
+    assert torch.equal(got.indices, want)
