@@ -432,9 +432,10 @@ int gpx_choice_logprobs_grad(gpx_ctx* ctx, const gpx_scores* scores, const int64
                              const void* d_logprobs, const void* d_grad_logprobs, int top, const int64_t* d_top_indices,
                              const void* d_grad_top, const void* d_entropy, const void* d_stats, const void* d_grad_entropy,
                              const void* d_grad_logsumexp, void* d_grad_scores, void* stream);
-/* Weight that each candidate of each pool has gathered: out = decay * weights + sum over the pool's rows of
- * row_weight * p (pools x candidates, contiguous; weights NULL, or a decay of 0: zeros; row_weights pools x rows contiguous, NULL: ones; a row
- * of weight 0 is not read).  out may be weights.  The sums have a fixed order.  Workspace as above. */
+/* Weight that each candidate of each pool has gathered: out = decay * weights + sum over the pool's rows of row_weight * p
+ * (pools x candidates, contiguous; weights NULL, or a decay of 0: zeros).  row_weights: pools x rows, contiguous, NULL: ones; a
+ * row of weight 0 is not read.  out may be weights, and overlaps nothing else.  The sums have a fixed order.  At most 65535
+ * pools.  Workspace as above. */
 int64_t gpx_pool_weights_workspace(int64_t pools, int64_t rows, int64_t candidates, int dtype);
 int gpx_pool_weights(gpx_ctx* ctx, const gpx_scores* scores, const void* d_row_weights, const void* d_weights, double decay,
                      void* d_out, void* d_workspace, int64_t workspace_bytes, void* stream);
