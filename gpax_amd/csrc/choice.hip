@@ -2,7 +2,7 @@
 // exponentials and the best alternatives of every row in ONE pass over the scores, and the gradient of all of them.
 //
 // Bound by memory for large pools (a score is read once; 3 - 4 fused operations and one exponential each) and by latency for
-// small ones: 2048 x 65536 bfloat16 take 47 us (5.7 TB/s) without alternatives, 67 with 20 and 92 with 64 of them (then
+// small ones: 2048 x 65536 bfloat16 take 47 us (5.7 TB/s) without alternatives, 67 with 20 and 90 with 64 of them (then
 // the vector units are busy 85 % of the time: 16 instructions a score, of them 9 for the sums); 1000 x 1024 float64 5 and, with 8, 8.7 us;
 // 1 x 201 4 and 5.7 us, of which an empty launch is 4.  A row is worked on by 1, 4 or 16 waves of one workgroup, or by several workgroups whose partial results a
 // second launch joins: as many waves as it takes to occupy the chip, no more (choice_plan).
@@ -109,6 +109,15 @@ __device__ __forceinline__ float least_of_order(uint32_t t, float) {
 __device__ __forceinline__ uint32_t low_order(double v) {
   const uint32_t u = (uint32_t)__double2loint(v);
   return __double2hiint(v) < 0 ? ~u : u;
+}
+// the next number above v (which is not NaN): x > v is x >= that
+__device__ __forceinline__ float next_above(float v) {
+  const int u = __float_as_int(v);
+  return __int_as_float(v == 0.0f ? 1 : u < 0 ? u - 1 : u + 1);
+}
+__device__ __forceinline__ double next_above(double v) {
+  const long long u = __double_as_longlong(v);
+  return __longlong_as_double(v == 0.0 ? 1ll : u < 0 ? u - 1 : u + 1);
 }
 template <typename A, int V>
 __device__ __forceinline__ A kth_of(const A (&v)[V], int k) {
@@ -272,9 +281,9 @@ struct Waiting {
     // above the list's own threshold strictly: a score equal to its k-th loses to it, whose index is lower (a wave takes its
     // steps in order); at or above the shared one, whose index may be anything
     const A own = list.thr_key;
-    const uint64_t better = __ballot(cm > own && cm >= shared);
+    A bound = own >= shared ? next_above(own) : shared; // one comparison a score
+    const uint64_t better = __ballot(cm >= bound);
     if (better == 0) return;
-    A bound = shared;
     const bool many = __popcll(better) >= (list.k > 32 ? list.k : 32);
     if (many) {
       A kth;
@@ -301,11 +310,11 @@ struct Waiting {
         A gm = x[g];
 #pragma unroll
         for (int e = g + 1; e < g + GROUP; ++e) gm = fmax(gm, x[e]);
-        if (__ballot(gm > own && gm >= bound) == 0) continue;
+        if (__ballot(gm >= bound) == 0) continue;
       }
 #pragma unroll
       for (int e = g; e < g + GROUP; ++e) {
-        const bool in = x[e] > own && x[e] >= bound;
+        const bool in = x[e] >= bound;
         const uint64_t mask = __ballot(in);
         if (mask) {
           const int at = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));

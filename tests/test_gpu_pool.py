@@ -625,3 +625,18 @@ def test_evict_from_forty_million():
     got = acq.pool_evict(w, 1000)
     want = torch.sort(torch.topk(w, 1000).indices).values
     assert torch.equal(got.indices, want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("shape", [(4, 200), (3, 1024), (2, 20000), (2, 70001)], ids=str)
+def test_alternatives_around_zero(kind, shape):
+    """Zeros of both signs and the smallest numbers there are, among the largest and the lowest ones."""
+    rng = np.random.default_rng(shape[1])
+    info = torch.finfo(getattr(torch, kind))
+    tiny = {"float64": 5e-324, "float32": 2.0 ** -149, "bfloat16": 2.0 ** -133, "float16": 2.0 ** -24}[kind]
+    for pool in ([0.0, -0.0, -1.0], [0.0, -0.0, tiny, -tiny, 2 * tiny, -1.0], [-tiny, -2 * tiny, -3 * tiny, info.min], [info.max, info.min, 0.0, tiny]):
+        for rare in (False, True):  # all of them often, or the last one nearly everywhere
+            p = None if not rare else np.r_[np.full(len(pool) - 1, 0.01), 1 - 0.01 * (len(pool) - 1)]
+            x = torch.as_tensor(rng.choice(np.array(pool), shape, p=p), device="cuda").to(getattr(torch, kind))
+            for top in (1, 20, 64):
+                np.testing.assert_array_equal(host(acq.choice_logprobs(x, top=top).top_indices), ref.choice(host(x), top=top)["top_indices"])
