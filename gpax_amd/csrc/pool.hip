@@ -86,10 +86,10 @@ __global__ __launch_bounds__(TEAMS * 64) void pool_weights_wave_kernel(WeightArg
     s = wave_sum(s);
     if (s == (A)0) continue; // nothing in this row may be chosen
     const A f = u / s;
-    if (f != f) { // NaN for what may be chosen, nothing for what may not
+    if (!(fabs(f) < (A)INFINITY)) { // infinite or NaN for what may be chosen, nothing for what may not (0 f would be NaN)
       load_step<T, VEC, U>(v, 0, SPAN, lane * VEC, x);
 #pragma unroll
-      for (int e = 0; e < PER_LANE; ++e) acc[e] += x[e] == neg_inf<A>() ? (A)0 : f;
+      for (int e = 0; e < PER_LANE; ++e) acc[e] += x[e] == neg_inf<A>() ? (A)0 : exp2_acc((x[e] - ref) * c) * f;
     } else {
 #pragma unroll
       for (int w = 0; w < U; ++w) {
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(WAVES * 64) void pool_weights_kernel(WeightArgs a) 
       for (int w = 0; w < WAVES; ++w) m = fmax(m, red[0][w]);
       const A ref = finite_max(m);
       A s = (A)0;
-      uint32_t there = 0; // which of this lane's candidates exist, for a row that is NaN
+      uint32_t there = 0; // which of this lane's candidates exist, for a row that is not finite
 #pragma unroll
       for (int w = 0; w < U; ++w) {
         if (w * SPAN >= n) break; // uniform
@@ -210,9 +210,9 @@ __global__ __launch_bounds__(WAVES * 64) void pool_weights_kernel(WeightArgs a) 
       for (int w = 0; w < WAVES; ++w) s += red[1][w];
       if (s == (A)0) continue; // nothing in this row may be chosen
       const A f = u / s;
-      if (f != f) { // NaN for what may be chosen, nothing for what may not
+      if (!(fabs(f) < (A)INFINITY)) { // infinite or NaN for what may be chosen, nothing for what may not (0 f would be NaN)
 #pragma unroll
-        for (int e = 0; e < PER_LANE; ++e) acc[e] += (there >> e) & 1 ? f : (A)0;
+        for (int e = 0; e < PER_LANE; ++e) acc[e] += (there >> e) & 1 ? x[e] * f : (A)0;
       } else {
 #pragma unroll
         for (int w = 0; w < U; ++w) {
