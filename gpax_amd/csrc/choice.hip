@@ -32,6 +32,7 @@ struct ChoiceArgs {
   int C;
   int top;
   int splits; // workgroups per row
+  const void* row_weights; // rows, or nullptr: a row of weight 0 is not read, and has the statistics of an empty one
   void *logprobs, *entropy, *lse, *stats, *top_logprobs;
   int64_t* top_indices;
   void* ws;
@@ -434,7 +435,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, sizeof(T) == 8 || WA
   if (row >= a.sc.rows) return; // WAVES == 1: whole waves, and no barrier below
   const int64_t b = (uint32_t)row / (uint32_t)a.sc.R, r = row - b * a.sc.R; // at most 2^25 rows
   const A c = temperature_scale(row_temperature<A>(a.sc, b, r));
-  const Row<T> v = row_view<T>(a.sc, b, r);
+  Row<T> v = row_view<T>(a.sc, b, r);
+  if (!TOP && a.row_weights && static_cast<const A*>(a.row_weights)[row] == (A)0) v.n = 0;
   Stats<A> st = stats_empty<A>();
   TopList<A> list;
   if (TOP) list.init(a.top);
@@ -723,11 +725,13 @@ int pool_scores_view(gpx_ctx* ctx, const gpx_scores* x, PoolScores* out, const c
 }
 
 int64_t row_stats_workspace(int64_t rows, int64_t M, int dtype) { return choice_workspace(rows, M, dtype, 0); }
-int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, void* d_stats, void* d_parts, int* splits, hipStream_t st) {
+int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, const void* d_row_weights, void* d_stats, void* d_parts, int* splits,
+                     hipStream_t st) {
   ChoiceArgs a{};
   const ChoicePlan p = choice_plan(sc.rows, sc.M);
   a.sc = sc;
   a.splits = p.splits;
+  a.row_weights = d_row_weights;
   a.stats = d_stats;
   a.ws = d_parts;
   *splits = p.splits;

@@ -446,8 +446,9 @@ struct DeviceGuard { // the caller's current device comes back whatever happens
   DeviceGuard& operator=(const DeviceGuard&) = delete;
 };
 // Statistics of every row, pass one of pool_weights over pools too long for a workgroup (choice.hip): rows x {m, log2 s} in
-// d_stats if *splits comes back as 1, else partial results of *splits parts of each row in d_parts
-int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, void* d_stats, void* d_parts, int* splits, hipStream_t st);
+// d_stats if *splits comes back as 1, else partial results of *splits parts of each row in d_parts; rows of weight 0 as empty ones
+int launch_row_stats(gpx_ctx* ctx, const PoolScores& sc, int dtype, const void* d_row_weights, void* d_stats, void* d_parts, int* splits,
+                     hipStream_t st);
 int64_t row_stats_workspace(int64_t rows, int64_t M, int dtype);
 
 } // namespace gpx

@@ -1214,7 +1214,7 @@ int gpx_pool_weights(gpx_ctx* ctx, const gpx_scores* scores, const void* d_row_w
   GPX_HIP(ctx, g.err);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (!p.one_pass && a.sc.rows > 0)
-    GPX_TRY(launch_row_stats(ctx, a.sc, scores->dtype, const_cast<void*>(a.stats), const_cast<void*>(a.parts), &a.splits, st));
+    GPX_TRY(launch_row_stats(ctx, a.sc, scores->dtype, a.row_weights, const_cast<void*>(a.stats), const_cast<void*>(a.parts), &a.splits, st));
   switch (scores->dtype) {
     case GPX_DTYPE_F64: weights_launch<double>(a, p, scores->pools, st); break;
     case GPX_DTYPE_F32: weights_launch<float>(a, p, scores->pools, st); break;

@@ -42,3 +42,35 @@ def test_row_weights_that_are_not_finite(kind, M, strided, weight):
     # each of two terms: the error of its exponent (|z| below 8, 8 u 16), of the sum of M terms and of 4 roundings; two additions
     tol = ref.U[kind] * (200 + M / 64 + 8 * 16 + 8) * np.abs(want[~there])
     assert np.all(np.abs(got[~there] - want[~there]) <= tol)
+
+
+NAMES = ("d_scores pools rows candidates x0 x1 x2 d_mask m0 m1 m2 d_lengths l0 l1 d_temperatures t0 t1 temperature dtype "
+         "lengths_64").split()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,M", [(37, 40000), (600, 20000), (4100, 16500)], ids=str)
+def test_rows_of_weight_0_are_not_read(kind, rows, M):
+    """Pools that take two passes, with several workgroups, one, and one wave a row: nothing of such a row (its scores are 1000,
+    the others below 40) gets into the statistics that the first pass leaves in the workspace."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.empty(rows, M, device="cuda").normal_(generator=g).clamp_(-40, 40).to(getattr(torch, kind))
+    u = torch.rand(rows, device="cuda", generator=g, dtype=ACC[kind]) + 0.5
+    u[1::3], x[1::3] = 0, 1000.0
+    eng, dtype = _lib.get_device_engine(0), KINDS.index(kind)
+    nbytes = _lib.load_library().gpx_pool_weights_workspace(1, rows, M, dtype)
+    ws = torch.zeros(nbytes, dtype=torch.uint8, device="cuda")
+    out = torch.empty(M, device="cuda", dtype=ACC[kind])
+    fields = dict(d_scores=x.data_ptr(), pools=1, rows=rows, candidates=M, x1=M, x2=1, temperature=1.0, dtype=dtype)
+    eng.pool_weights(_lib.POOL_SCORES.pack(*[fields.get(n, 0) for n in NAMES]), u.data_ptr(), 0, 0.0, out.data_ptr(), ws.data_ptr(),
+                     nbytes, torch.cuda.current_stream().cuda_stream)
+    left = ws[:nbytes // 8 * 8].view(ACC[kind])
+    assert not (left == 1000.0).any()
+    assert torch.equal(out, acq.pool_weights(x, row_weights=u))
+    x[1::3] = math.nan
+    assert torch.equal(out, acq.pool_weights(x, row_weights=u))
+    z = x[u != 0].double()
+    e = torch.exp(z - z.amax(1, keepdim=True))
+    want = (u[u != 0].double()[:, None] * (e / e.sum(1, keepdim=True))).sum(0)
+    # as for other weights: the error of an exponent with |z| below 40, the sum of M terms, 4 roundings, an addition a row
+    assert torch.all((out.double() - want).abs() <= ref.U[kind] * (200 + M / 64 + 8 * 80 + 8 + rows) * want)
