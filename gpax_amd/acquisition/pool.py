@@ -286,7 +286,7 @@ class _Policy:
             T = 1.0
             self.temps = t = space.take(temperature, "temperature", (acc,))
             ts = _pad2(_broadcast_strides(tuple(t.shape), space.strides(t), lead, "temperature"))
-            if space.host and not (np.all(t > 0) and np.all(np.isfinite(t))):
+            if space.host and not (np.all(t >= np.finfo(acc).tiny) and np.all(np.isfinite(t))):  # 1 / T must be finite too
                 raise ValueError("the temperature must be positive and finite")
         self._fields = (p, r, M, *_pad3(space.strides(x))), ms, ls, (*ts, T, _DTYPES[kind], n64)
 
@@ -339,8 +339,9 @@ def choice_logprobs(scores, choices=None, *, temperature=1.0, mask=None, lengths
         choices: the candidates whose log probabilities are wanted, shape scores.shape[:-1] (one a row) or
             scores.shape[:-1] + (C,); -1 is a filler (log probability 0), a candidate that does not exist has -inf
             (a number outside the pool: ValueError for NumPy arrays, NaN for tensors)
-        temperature: T, a number or an array broadcast to the rows (of the accumulator's type); positive and finite
-            (anything else: ValueError for numbers and NumPy arrays, a row of NaN for tensors)
+        temperature: T, a number or an array broadcast to the rows (of the accumulator's type); positive, finite and not
+            subnormal (anything else: ValueError for numbers and NumPy arrays; for tensors a row of NaN where it is not positive
+            or log2(e) / T is not finite)
         mask: which candidates may be chosen, bool or uint8, broadcast to the scores
         lengths: how many candidates each row has, int64 or int32, broadcast to the rows (clamped to 0 .. M)
         top: number of best alternatives to return, at most 64

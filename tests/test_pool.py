@@ -225,3 +225,18 @@ def test_no_scalar_move_has_a_literal_of_more_than_32_bits(source, tmp_path):
     assert "s_endpgm" in text
     bad = [m for m in re.findall(r"[sv]_mov_b64(?:_e32)? [sv]\[[0-9:]+\], (-?(?:0x[0-9a-f]+|[0-9]+))", text) if not -2 ** 31 <= int(m, 0) < 2 ** 32]
     assert not bad, bad
+
+
+@pytest.mark.parametrize("kind,T", [("float32", 1e-39), ("float16", 1e-39), ("float32", 1e-45), ("float64", 1e-310), ("float64", 5e-324)])
+def test_temperatures_too_small_to_divide_by(kind, T):
+    """A positive number below the type's normal ones is refused in an array as it is alone: 1 / T may be infinite."""
+    x = np.zeros((3, 10), dtype=kind)
+    temps = np.ones(3, dtype="float64" if kind == "float64" else "float32")
+    temps[1] = T
+    assert 0 < temps[1] < np.finfo(temps.dtype).tiny
+    for t in (T, temps, temps[1:2]):
+        for call in (acq.choice_logprobs, acq.pool_weights):
+            with pytest.raises(ValueError):
+                call(x, temperature=t)
+    temps[1] = np.finfo(temps.dtype).tiny
+    assert np.all(acq.choice_logprobs(x, temperature=temps).entropy > 2)
