@@ -8,7 +8,7 @@ Arguments are either all NumPy arrays, which are staged through the default engi
 all torch tensors on one GPU, which are worked on in place on torch's current stream, without a copy and without waiting
 (import torch before the library is loaded, so that both use one HIP runtime; the first call on a GPU makes its context and
 must not be inside a graph capture).  No autograd graph is recorded: `choice_logprobs_grad` is the backward pass, and a
-tensor that requires grad is refused while gradients are enabled.
+tensor that requires grad is refused while gradients are enabled, one with a forward-mode tangent always.
 
 Scores are (M,), (rows, M) or (pools, rows, M), of any strides, in float64, float32, bfloat16 or float16.  Sums,
 statistics and all real results but gradients are float64 for float64 scores and float32 for the others.  A candidate
@@ -76,10 +76,11 @@ _torch = None  # torch, its types and the address of a stream, once a tensor has
 _kind_of: dict = {}
 _type_of: dict = {}
 _stream_of = None
+_forward_ad = None
 
 
 def _bind_torch() -> None:
-    global _torch, _stream_of
+    global _torch, _stream_of, _forward_ad
     torch = sys.modules["torch"]
     if not _one_runtime():
         raise _lib.GpxError("libgpx and torch have loaded two HIP runtimes: import torch before gpax_amd's library is loaded "
@@ -89,6 +90,7 @@ def _bind_torch() -> None:
         _kind_of[_type_of[name]] = name
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # current_stream() without making a Stream object of it
     _stream_of = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _forward_ad = torch.autograd.forward_ad
     _torch = torch
 
 
@@ -114,6 +116,8 @@ class _Device:
             raise ValueError(f"{name} has dtype {a.dtype}; expected {' or '.join(kinds)}")
         if a.requires_grad and _torch.is_grad_enabled():
             raise ValueError(f"{name} requires grad, and no graph is recorded: detach it and call choice_logprobs_grad")
+        if getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(a).tangent is not None:
+            raise ValueError(f"{name} has a tangent, which forward mode would lose here: pass its primal")
         if a.is_neg() or a.is_conj():
             a = a.resolve_conj().resolve_neg()
         return a.contiguous() if contiguous else a

@@ -74,3 +74,27 @@ def test_rows_of_weight_0_are_not_read(kind, rows, M):
     want = (u[u != 0].double()[:, None] * (e / e.sum(1, keepdim=True))).sum(0)
     # as for other weights: the error of an exponent with |z| below 40, the sum of M terms, 4 roundings, an addition a row
     assert torch.all((out.double() - want).abs() <= ref.U[kind] * (200 + M / 64 + 8 * 80 + 8 + rows) * want)
+
+
+def test_tangents_are_refused():
+    """Forward mode would lose them: no result has one."""
+    from torch.autograd import forward_ad
+    x, w = torch.randn(3, 10, device="cuda"), torch.rand(10, device="cuda")
+    c = torch.zeros(3, 1, device="cuda", dtype=torch.int64)
+    want = acq.choice_logprobs(x, c, top=2)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        dx, dw = dual(x), dual(w)
+        assert not dx.requires_grad
+        for call in [lambda: acq.choice_logprobs(dx, c), lambda: acq.choice_logprobs(x, temperature=dual(torch.ones(3, device="cuda"))),
+                     lambda: acq.choice_logprobs_grad(x, want, c, grad_entropy=dual(torch.ones(3, device="cuda"))), lambda: acq.pool_weights(dx),
+                     lambda: acq.pool_weights(x, dw), lambda: acq.pool_weights(x, out=dw), lambda: acq.pool_evict(dw, 4),
+                     lambda: acq.pool_evict(w, 4, (dual(torch.rand(10, 2, device="cuda")),))]:
+            with pytest.raises(ValueError):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError):
+                call()
+        plain = acq.choice_logprobs(forward_ad.unpack_dual(dx).primal, c, top=2)  # no tangent: as ever
+        assert acq.pool_evict(w, 4, (c.expand(3, 10).t(),)).indices.shape == (4,)
+    for a, b in zip(want, plain):
+        assert torch.equal(a, b)
