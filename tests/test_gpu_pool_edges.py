@@ -98,3 +98,15 @@ def test_tangents_are_refused():
         assert acq.pool_evict(w, 4, (c.expand(3, 10).t(),)).indices.shape == (4,)
     for a, b in zip(want, plain):
         assert torch.equal(a, b)
+
+
+def test_out_may_lie_in_no_argument():
+    """Temperatures, lengths and row weights of the same storage as `out`, behind its first element and before its last."""
+    x = torch.randn(4, 64, device="cuda")
+    room = torch.ones(80, device="cuda")
+    ints = room.view(torch.int32)
+    for kw in [dict(temperature=room[60:64]), dict(temperature=room[:1]), dict(row_weights=room[63:67]), dict(lengths=ints[60:64]), dict(lengths=ints[:1]),
+               dict(temperature=room[::21][:4]), dict(lengths=room.view(torch.int64)[30:34])]:
+        with pytest.raises(ValueError, match="overlaps"):
+            acq.pool_weights(x, out=room[:64], **kw)
+    assert acq.pool_weights(x, temperature=room[64:68], row_weights=room[68:72], lengths=ints[72:76], out=room[:64]).data_ptr() == room.data_ptr()
