@@ -111,7 +111,10 @@ def _gathered_weights(rng_key, model, X, temperature, maximize, n, noiseless, we
     X = X[:, None] if X.ndim < 2 else X
     if getattr(model, "mcmc", None) is not None:
         _, y_sampled = model.predict(rng_key, X, n=n, noiseless=noiseless, **kwargs)
-        draws = np.asarray(y_sampled).reshape(-1, X.shape[0])
+        draws = np.asarray(y_sampled)
+        if draws.ndim > 3 or draws.shape[-1] != len(X):  # vExactGP: (samples, n, tasks, M)
+            raise ValueError(f"draws have shape {draws.shape}; expected one value for each of the {len(X)} points, of a single task")
+        draws = draws.reshape(-1, len(X))
     else:
         draws = _vi_draws(rng_from_key(rng_key), model, X, n, noiseless, **kwargs)
     counts = np.isfinite(draws).all(axis=1)  # a posterior sample whose factorisation failed has NaN draws: it has no say
@@ -124,7 +127,7 @@ def PBest(rng_key, model, X, temperature: float = 0.1, maximize: bool = False, n
     """Probability of being the best candidate, as the softmax of every posterior draw over X at the given temperature (in
     units of y; towards 0: the share of draws whose extremum each candidate is) gives it, averaged over the draws: n per
     posterior sample (HMC) or n at the point estimate (VI).  What Thompson sampling (acquisition.py:488-524) picks from, one
-    draw at a time."""
+    draw at a time.  For models of a single target: vector-valued ones (vExactGP) are refused."""
     _, w, count = _gathered_weights(rng_key, model, X, temperature, maximize, n, noiseless, None, 1.0, kwargs)
     return w / count if count else np.full(len(w), np.nan)
 

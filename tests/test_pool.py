@@ -240,3 +240,22 @@ def test_temperatures_too_small_to_divide_by(kind, T):
                 call(x, temperature=t)
     temps[1] = np.finfo(temps.dtype).tiny
     assert np.all(acq.choice_logprobs(x, temperature=temps).entropy > 2)
+
+
+@pytest.mark.parametrize("tasks", [1, 2, 4])
+def test_models_of_several_targets_are_refused(tasks):
+    """A vector-valued model draws (samples, n, tasks, M) at X of (tasks, M, d): cut into rows of X's length, they would weigh the
+    tasks instead of the candidates."""
+    import bench_inputs
+    from gpax_amd.models import vExactGP
+    from gpax_amd.utils import get_keys
+    Xt, y, Xn, _ = bench_inputs.synthetic_problem(12, 1, 8, seed=2)
+    m = vExactGP(1, "RBF")
+    m.fit(get_keys()[0], np.stack([Xt] * tasks), np.stack([y + t for t in range(tasks)]), num_warmup=4, num_samples=4, progress_bar=False,
+          print_summary=False)
+    Xn = np.stack([Xn] * tasks)
+    assert m.predict(get_keys()[1], Xn, n=2)[1].shape == (4, 2, tasks, 8)
+    for X in (Xn, Xn[..., 0]):
+        for call in (lambda: acq.PBest(get_keys()[1], m, X, n=2), lambda: acq.shrink_pool(get_keys()[1], m, X, 1)):
+            with pytest.raises(ValueError):
+                call()
