@@ -358,6 +358,14 @@ __device__ __forceinline__ A common_threshold(A most, int k, WaveShare<A, W>& sh
   return kth_of(top, k);
 }
 
+// (x - m) / T - log s.  Not through powers of two: a lowest score overflows there.  A difference of a whole range overflows too,
+// and need not once it is divided.
+template <typename A>
+__device__ __forceinline__ A log_prob(A x, A m, A T, A log_s) {
+  const A d = x - m;
+  return (d == neg_inf<A>() ? x / T - m / T : d / T) - log_s;
+}
+
 // What a row's statistics are turned into, by a team of `size` threads of which this one is `at`; the list by its wave.
 template <typename T>
 __device__ __forceinline__ void finish_row(const ChoiceArgs& a, int64_t row, int64_t b, int64_t r, const Stats<typename Acc<T>::type>& st, int at,
@@ -381,7 +389,7 @@ __device__ __forceinline__ void finish_row(const ChoiceArgs& a, int64_t row, int
         lp = (A)NAN; // no candidate of this pool: never read
       } else if (j >= 0) {
         const A x = row_at(v, (int)j);
-        lp = x == neg_inf<A>() ? x : (x - st.m) / T_row - log_s; // not through powers of two: a lowest score overflows there
+        lp = x == neg_inf<A>() ? x : log_prob(x, st.m, T_row, log_s);
       }
       static_cast<A*>(a.logprobs)[row * a.C + q] = lp;
     }
@@ -393,7 +401,7 @@ __device__ __forceinline__ void finish_top(const ChoiceArgs& a, int64_t row, int
   const bool there = list.idx != 0xffffffffu;
   a.top_indices[row * a.top + lane] = there ? (int64_t)list.idx : -1;
   static_cast<A*>(a.top_logprobs)[row * a.top + lane] =
-      there ? (list.key - st.m) / row_temperature<A>(a.sc, b, r) - ln2<A>() * log2_acc(st.s) : neg_inf<A>();
+      there ? log_prob(list.key, st.m, row_temperature<A>(a.sc, b, r), ln2<A>() * log2_acc(st.s)) : neg_inf<A>();
 }
 
 // Joins the statistics and lists of the W waves of a workgroup: log2 W rounds, each wave with the one `half` above it.

@@ -394,7 +394,8 @@ int gpx_potrf(gpx_ctx* ctx, int n, const double* A, double* L, int* info);
  * accumulator's type").  A candidate exists for a row if it lies below the row's length, its mask byte is nonzero and its
  * score is not -inf; what is stored in the other places is never used.  A row in which nothing exists has log probabilities
  * -inf, entropy 0, log-sum-exp -inf, no alternatives, gradient 0 and adds no weight.  A NaN or +inf score that exists, or a
- * temperature on the device that is not positive and finite, or so small that log2(e) / T is not, makes its row NaN. */
+ * temperature on the device that is not positive and finite, or so small that log2(e) / T is not, makes its row NaN.
+ * A score that lies farther below its row's largest than the accumulator's type reaches has probability 0 at any temperature. */
 #define GPX_DTYPE_F64 0
 #define GPX_DTYPE_F32 1
 #define GPX_DTYPE_BF16 2

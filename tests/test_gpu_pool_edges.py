@@ -110,3 +110,28 @@ def test_out_may_lie_in_no_argument():
         with pytest.raises(ValueError, match="overlaps"):
             acq.pool_weights(x, out=room[:64], **kw)
     assert acq.pool_weights(x, temperature=room[64:68], row_weights=room[68:72], lengths=ints[72:76], out=room[:64]).data_ptr() == room.data_ptr()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("M", [3, 1000, 5000, 70001])
+def test_log_probabilities_of_scores_a_whole_range_apart(kind, M):
+    """The largest and the lowest number there are, over T = 8: their difference is infinite in the accumulator's type, the log
+    probability is not.  Only three candidates exist: p = 1, 0, 0 in any type."""
+    big = torch.finfo(getattr(torch, kind)).max
+    x = torch.zeros(2, M, device="cuda", dtype=getattr(torch, kind))
+    x[:, 0], x[:, M // 2], x[:, M - 1] = big, 0, -big
+    mask = torch.zeros(M, device="cuda", dtype=torch.bool)
+    mask[[0, M // 2, M - 1]] = True
+    c = torch.tensor([[0, M // 2, M - 1, -1]] * 2, device="cuda")
+    r = acq.choice_logprobs(x, c, temperature=8.0, mask=mask, top=3)
+    want = np.array([[0.0, -(big / 8), -(big / 4), 0.0]] * 2)
+    # each score by T, their difference, the logarithm of the sum: a rounding each
+    assert np.all(np.abs(host(r.logprobs) - want) <= 4 * ref.U[kind] * np.abs(want))
+    assert np.all(np.abs(host(r.top_logprobs) - want[:, :3]) <= 4 * ref.U[kind] * np.abs(want[:, :3]))
+    assert r.top_indices.tolist() == [[0, M // 2, M - 1]] * 2
+    g = torch.tensor([[0.0, 0.0, 4.0, 9.0]] * 2, device="cuda", dtype=ACC[kind])
+    d = host(acq.choice_logprobs_grad(x, r, c, grad_logprobs=g, temperature=8.0, mask=mask))
+    full = np.zeros((2, M))
+    full[:, 0] -= 0.5
+    full[:, M - 1] += 0.5  # (1 - p) g / T, and -p g / T
+    np.testing.assert_array_equal(d, full)
