@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256) void pool_weights_join_kernel(WeightArgs a) {
 // One workgroup per pool where the pool fits its registers (16384 candidates).  Longer pools are cut into chunks of 4096, a
 // workgroup each, over six launches: range of the keys | histograms of 12, 12 and 12 bits | the few candidates that share all
 // 36 (or that need no telling apart) | output.  Read six times, but 2 MB of weights stay in the caches: bound by the launches.
-// 64-bit weights of more than THREE_DIGITS_MAX candidates have a histogram for every 12 bits of a key.
+// 64-bit weights of many or very long pools (REREADS_MAX) have a histogram for every 12 bits of a key.
 
 constexpr int EVICT_PAYLOADS = 16;
 // Payload rows up to this are moved by the lane that keeps the candidate, longer ones by a launch of their own: of 64 pools of
@@ -710,10 +710,13 @@ __global__ __launch_bounds__(1024) void pool_evict_kernel(EvictArgs a) {
 constexpr int CHUNK_PER = 4, CHUNK = 1024 * CHUNK_PER;
 constexpr int MAX_TIED = 1024; // candidates told apart one by one in the last launch
 // Three digits are all of a 32-bit key.  Of a 64-bit one they leave those that agree in 36 bits, counted from the highest that
-// differs, to the last launch; if those are many, each workgroup goes through the whole pool, 0.4 ms at 262144 candidates and 1.3
-// at this size, growing with the square.  (After two digits that already happens to weights within 2^-14 of each other beside
-// one that is larger; the third launch costs 3 us.)  Beyond it a launch for every digit that a key has.
-constexpr int64_t THREE_DIGITS_MAX = 1 << 19;
+// differs, to the last launch; if those are many, the workgroup of each chunk goes through all chunks of its pool.  (After two
+// digits that already happens to weights within 2^-14 of each other beside one that is larger; the third launch costs 3 us.)  Up
+// to this many chunks read by all workgroups together (one pool of 2^19 candidates, 64 of 65536) that is accepted; beyond it
+// there is a launch for every digit that a key has.  Ordinary weights, and weights that all agree in 36 bits beside one that does
+// not, with three digits and with six: 1 x 262144 35 and 240 us, 42 and 58; 1 x 524288 36 and 493, 43 and 61; 64 x 65536 93 and
+// 470, 103 and 164; 64 x 131072 172 and 1546, 188 and 300; 64 x 524288 674 and 19032, 741 and 1162.
+constexpr int64_t REREADS_MAX = 128 * 128;
 template <typename Key>
 constexpr int DIGITS = (8 * (int)sizeof(Key) + WIDE_BITS - 1) / WIDE_BITS;
 
@@ -841,6 +844,18 @@ __global__ __launch_bounds__(1024) void pool_evict_hist_kernel(EvictArgs a, int 
   const int64_t b = blockIdx.y, c = blockIdx.x;
   const PoolCut cut = pool_cut(a, b);
   const EvictView<Key> v = evict_view<Key>(a, b);
+  if (!FIRST && level > DIGITS<uint32_t>) { // digits that few pools need: not read where nothing was left to decide a launch ago
+    const Prefix<Key> q{v.st->prefix[level - 2], v.st->shift[level - 2], v.st->need[level - 2], v.st->count[level - 2]};
+    if (q.shift == 0 || q.need == 0 || q.need == q.count) {
+      if (c == 0 && threadIdx.x == 0) {
+        v.st->prefix[level - 1] = q.prefix;
+        v.st->shift[level - 1] = q.shift;
+        v.st->need[level - 1] = q.need;
+        v.st->count[level - 1] = q.count;
+      }
+      return;
+    }
+  }
   Chunk<W> k;
   k.load(a, cut, b, c * CHUNK);
   const Prefix<Key> p = advance_prefix<Key, FIRST>(a, v, cut, level, sh_keys);
@@ -1257,7 +1272,7 @@ int gpx_pool_evict(gpx_ctx* ctx, int dtype, int64_t pools, int64_t candidates, c
   a.out = d_weights_out;
   a.ws = d_workspace;
   a.chunks = (candidates + CHUNK - 1) / CHUNK;
-  a.levels = dtype == GPX_DTYPE_F64 && candidates > THREE_DIGITS_MAX ? DIGITS<uint64_t> : DIGITS<uint32_t>;
+  a.levels = dtype == GPX_DTYPE_F64 && pools * a.chunks * a.chunks > REREADS_MAX ? DIGITS<uint64_t> : DIGITS<uint32_t>;
   for (int i = 0; i < npayload; ++i) {
     const int64_t rb = payload_row_bytes[i];
     if (rb == 0 || rb > FUSED_ROW_BYTES) continue;

@@ -135,3 +135,40 @@ def test_log_probabilities_of_scores_a_whole_range_apart(kind, M):
     full[:, 0] -= 0.5
     full[:, M - 1] += 0.5  # (1 - p) g / T, and -p g / T
     np.testing.assert_array_equal(d, full)
+
+
+def weights_that_agree(shape, g):
+    """Weights that agree in their 36 upper bits, all over the pools, beside one that does not."""
+    w = 1.0 + 1e-9 * torch.rand(shape, device="cuda", generator=g, dtype=torch.float64)
+    w[..., 7] = 100.0
+    return w
+
+
+@pytest.mark.parametrize("shape", [(64, 65536), (65, 65537), (5, 250001), (130, 40961), (3, 524288)], ids=str)
+def test_evict_from_several_long_pools_of_weights_that_agree(shape):
+    """On both sides of the rule for the number of digits, which looks at all pools."""
+    M, budget = shape[1], shape[1] // 3
+    g = torch.Generator(device="cuda").manual_seed(M)
+    w = weights_that_agree(shape, g)
+    lengths = torch.randint(budget, M + 1, shape[:1], device="cuda", generator=g)
+    got = acq.pool_evict(w, budget, first=3, recent=10, lengths=lengths)
+    for b, n in enumerate(lengths.tolist()):
+        order = torch.sort(w[b, 3:n - 10], descending=True, stable=True).indices[:budget - 13] + 3
+        keep = torch.cat([torch.arange(3, device="cuda"), torch.sort(order).values, torch.arange(n - 10, n, device="cuda")])
+        assert torch.equal(got.indices[b], keep if n > budget else torch.arange(budget, device="cuda"))
+
+
+def test_evict_of_many_long_pools_takes_no_time_in_squares():
+    """What agrees in its upper bits costs a few passes more, and not a pass for every chunk of 4096 (28 times as long here)."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    shape, times = (64, 524288), []
+    for w in (torch.rand(shape, device="cuda", generator=g, dtype=torch.float64), weights_that_agree(shape, g)):
+        acq.pool_evict(w, 100000)
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        for _ in range(3):
+            acq.pool_evict(w, 100000)
+        end.record()
+        end.synchronize()
+        times.append(start.elapsed_time(end))
+    assert times[1] < 6 * times[0], times
