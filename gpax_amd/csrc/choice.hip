@@ -2,9 +2,10 @@
 // exponentials and the best alternatives of every row in ONE pass over the scores, and the gradient of all of them.
 //
 // Bound by memory for large pools (a score is read once; 3 - 4 fused operations and one exponential each) and by latency for
-// small ones: 2048 x 65536 bfloat16 take 47 us (5.7 TB/s) without alternatives, 67 with 20 and 90 with 64 of them (then
-// the vector units are busy 85 % of the time: 16 instructions a score, of them 9 for the sums); 1000 x 1024 float64 5 and, with 8, 8.7 us;
-// 1 x 201 4 and 5.7 us, of which an empty launch is 4.  A row is worked on by 1, 4 or 16 waves of one workgroup, or by several workgroups whose partial results a
+// small ones: 2048 x 65536 bfloat16, three inputs in turn, take 53 us (5.1 TB/s) without alternatives, 66 with 20 and 88 with 64 of
+// them (one input again and again, partly in cache: 45, 63 and 86).  That is 10.8, 15.4 and 17.9 vector instructions a score, which
+// occupy the vector units for 75, 82 and 73 % of the time.  1000 x 1024 float64 take 5.4 and, with 8, 8.8 us; 1 x 201 4.0 and,
+// with one, 5.6 us, of which an empty launch is 4.  A row is worked on by 1, 4 or 16 waves of one workgroup, or by several workgroups whose partial results a
 // second launch joins: as many waves as it takes to occupy the chip, no more (choice_plan).
 //
 // Alternatives: every wave keeps the best 64 candidates it has met, one per lane, sorted by (score descending, index

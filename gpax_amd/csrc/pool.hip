@@ -119,8 +119,8 @@ __global__ __launch_bounds__(TEAMS * 64) void pool_weights_wave_kernel(WeightArg
 // sum.  What is needed of the rows (scale, weight, length) is fetched for 64 at a time, and the next row's scores are on their
 // way while one is worked on (DENSE: candidates, and mask bytes, side by side; else they are loaded where they are used).
 // One workgroup of 16 waves fills a CU's registers, so a row's two barriers and reductions stand in the open: 2048 x 16384
-// float32 take 32.7 us (4.1 TB/s; the vector units are busy half of it, 20 instructions a score), 16 x 128 x 16381 35 us, with
-// rows half as long on average 32, and 6 to join.  The two passes of longer pools would take 51 and 52.  4 waves up to 4096
+// float32 take 33.5 us (4.0 TB/s; 20 vector instructions a score occupy the vector units for 55 % of it, at 128 registers of which
+// 3 spill), 16 x 128 x 16381 35 us, with rows half as long on average 32, and 7 to join.  The two passes of longer pools would take 51 and 52.  4 waves up to 4096
 // candidates: 2000 x 4096 float32 12.6 us and 8.6 to join, with 16 waves 21.5 and 4.6; float64 1000 x 4096 17.3 against 19.6.
 constexpr int ROW_BLOCK = 64;
 template <typename A>
@@ -235,7 +235,8 @@ __global__ __launch_bounds__(WAVES * 64) void pool_weights_kernel(WeightArgs a) 
 // LDS; the next row that reaches into the tile is on its way while one is worked on; a mask that all rows share is read once.
 // A vector that would cross the end of the pool starts earlier, and only its own candidates are written.  DENSE: candidates (and
 // mask bytes) side by side.  64 x 262144 float64 with a shared mask: 36 us (3.7 TB/s, behind 28 us of the first pass), float32
-// 15.2 us (4.4 TB/s), bfloat16 16.4: exponentials and 64-bit arithmetic, then memory.
+// 15.6 us (4.3 TB/s), bfloat16 16.2: exponentials and 64-bit arithmetic (60 vector instructions a score in float64, which occupy
+// the vector units for 72 % of the time), then memory.
 constexpr int COL_BLOCK = 64;
 constexpr int col_vecs(int size) { return size == 2 ? 1 : 2; } // vectors a lane holds of a row (one is 8 scores of 16 bits)
 template <typename A>
