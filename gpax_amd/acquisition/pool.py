@@ -408,7 +408,7 @@ def choice_logprobs_grad(scores, forward: ChoiceLogprobs, choices=None, *, grad_
     if not isinstance(forward, ChoiceLogprobs):
         raise ValueError("forward must be what choice_logprobs returned")
     state = sp.take(forward.state, "forward.state", (acc,), contiguous=True)
-    if state.ndim != 1 or state.shape[0] < 4 * pol.pools * pol.rows:
+    if state.ndim != 1 or state.shape[0] < 4 * pol.pools * pol.rows or tuple(forward.entropy.shape) != pol.lead:
         raise ValueError("forward is not the forward call on these scores")
     logprobs = entropy = top_i = None
     g_lp = g_h = g_lse = g_top = None

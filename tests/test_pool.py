@@ -259,3 +259,15 @@ def test_models_of_several_targets_are_refused(tasks):
         for call in (lambda: acq.PBest(get_keys()[1], m, X, n=2), lambda: acq.shrink_pool(get_keys()[1], m, X, 1)):
             with pytest.raises(ValueError):
                 call()
+
+
+def test_gradient_of_a_forward_call_on_other_rows():
+    """Whichever gradient is given, `forward` has to be of the same rows."""
+    x = np.random.default_rng(0).standard_normal((4, 6))
+    r = acq.choice_logprobs(x, top=2)
+    for kw in [dict(), dict(grad_logsumexp=np.ones(2)), dict(grad_entropy=np.ones(2)), dict(grad_top_logprobs=np.ones((2, 2)))]:
+        with pytest.raises(ValueError):
+            acq.choice_logprobs_grad(x[:2], r, **kw)
+    with pytest.raises(ValueError):
+        acq.choice_logprobs_grad(x.reshape(2, 2, 6), r, grad_logsumexp=np.ones((2, 2)))
+    assert acq.choice_logprobs_grad(x, r, grad_logsumexp=np.ones(4)).shape == (4, 6)
