@@ -1255,6 +1255,7 @@ int gpx_pool_evict(gpx_ctx* ctx, int dtype, int64_t pools, int64_t candidates, c
   if (npayload < 0 || npayload > 16) return bad_arg(ctx, "gpx_pool_evict: at most 16 payload arrays");
   if (pools == 0) return 0;
   if ((!d_weights && candidates > 0) || !d_indices || !d_new_lengths || !d_weights_out) return bad_arg(ctx, "gpx_pool_evict: null pointer");
+  if (npayload > 0 && (!d_payload || !d_payload_out || !payload_row_bytes)) return bad_arg(ctx, "gpx_pool_evict: null payload arrays");
   for (int i = 0; i < npayload; ++i) {
     if (payload_row_bytes[i] < 0 || payload_row_bytes[i] > INT32_MAX) return bad_arg(ctx, "gpx_pool_evict: payload row size");
     if (payload_row_bytes[i] > 0 && ((!d_payload[i] && candidates > 0) || !d_payload_out[i])) return bad_arg(ctx, "gpx_pool_evict: null payload");

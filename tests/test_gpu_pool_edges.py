@@ -172,3 +172,12 @@ def test_evict_of_many_long_pools_takes_no_time_in_squares():
         end.synchronize()
         times.append(start.elapsed_time(end))
     assert times[1] < 6 * times[0], times
+
+
+def test_the_library_refuses_payload_without_its_arrays():
+    import ctypes as C
+    eng = _lib.get_device_engine(0)
+    arrays, sizes = (C.c_void_p * 1)(1), (C.c_int64 * 1)(8)
+    for args in [(None, arrays, sizes), (arrays, None, sizes), (arrays, arrays, None)]:
+        with pytest.raises(_lib.GpxError, match="payload"):
+            eng._check(eng._lib.gpx_pool_evict(eng._ctx, 0, 1, 8, 1, 0, 0, 0, 4, 0, 0, 1, 1, 1, 1, *args, 0, 0, 0), "gpx_pool_evict")
