@@ -5,8 +5,8 @@
 // small ones: 2048 x 65536 bfloat16, three inputs in turn, take 53 us (5.1 TB/s) without alternatives, 66 with 20 and 88 with 64 of
 // them (one input again and again, partly in cache: 45, 63 and 86).  That is 10.8, 15.4 and 17.9 vector instructions a score, which
 // occupy the vector units for 75, 82 and 73 % of the time.  1000 x 1024 float64 take 5.4 and, with 8, 8.8 us; 1 x 201 4.0 and,
-// with one, 5.6 us, of which an empty launch is 4.  A row is worked on by 1, 4 or 16 waves of one workgroup, or by several workgroups whose partial results a
-// second launch joins: as many waves as it takes to occupy the chip, no more (choice_plan).
+// with one, 5.6 us, of which an empty launch is 4.  A row is worked on by 1, 4 or 16 waves of one workgroup, or by several
+// workgroups whose partial results a second launch joins: as many waves as it takes to occupy the chip, no more (choice_plan).
 //
 // Alternatives: every wave keeps the best 64 candidates it has met, one per lane, sorted by (score descending, index
 // ascending).  The k-th of them is a threshold that few later candidates pass: a step whose largest score does not is left

@@ -119,9 +119,10 @@ __global__ __launch_bounds__(TEAMS * 64) void pool_weights_wave_kernel(WeightArg
 // sum.  What is needed of the rows (scale, weight, length) is fetched for 64 at a time, and the next row's scores are on their
 // way while one is worked on (DENSE: candidates, and mask bytes, side by side; else they are loaded where they are used).
 // One workgroup of 16 waves fills a CU's registers, so a row's two barriers and reductions stand in the open: 2048 x 16384
-// float32 take 33.5 us (4.0 TB/s; 20 vector instructions a score occupy the vector units for 55 % of it, at 128 registers of which
-// 3 spill), 16 x 128 x 16381 35 us, with rows half as long on average 32, and 7 to join.  The two passes of longer pools would take 51 and 52.  4 waves up to 4096
-// candidates: 2000 x 4096 float32 12.6 us and 8.6 to join, with 16 waves 21.5 and 4.6; float64 1000 x 4096 17.3 against 19.6.
+// float32 take 33.5 us (4.0 TB/s; 20 vector instructions a score occupy the vector units for 55 % of it; of its registers, 128 at
+// most, 3 spill), 16 x 128 x 16381 35 us, with rows half as long on average 32, and 7 to join.  The two passes of longer pools
+// would take 51 and 52.  4 waves up to 4096 candidates: 2000 x 4096 float32 12.6 us and 8.6 to join, with 16 waves 21.5 and 4.6;
+// float64 1000 x 4096 17.3 against 19.6.
 constexpr int ROW_BLOCK = 64;
 template <typename A>
 struct WorkRow {
